@@ -361,6 +361,104 @@ int mcc_adam_update_f32(void* stream, float* param, size_t param_nbytes, const f
                         float weight_decay);
 
 /*
+ * Row-wise operators around the counter layers: the norm in front of them, whose gain and bias the side
+ * optimizers train, and the log probabilities and the distillation loss behind the vocabulary head,
+ * whose gradient starts the backward pass.  The reference has a norm and a loss of its own among its
+ * general ops (src/ops/norm.cpp, src/ops/loss.cpp); these are no replacements of them call by call.
+ *
+ * Large tensors are rows of elements of one type, MCC_ELEMENT_*, aligned to the element; a stride counts
+ * the elements from the start of a row to that of the next (at least the row's length).  Whatever the
+ * type, everything is computed in binary32 and a result is rounded to the type once.  An output may
+ * replace an input of the same type where that is said (same pointer, same stride); any other overlap of
+ * the large tensors is refused.  Equal calls give equal bytes.  Rows hold at most 2^30 elements.
+ * Nothing is allocated and nothing is kept between calls: all entry points may be captured into a graph.
+ * Workspaces are aligned to 16 bytes and belong to the call until it has run; their sizes depend on the
+ * arguments of the query alone and may be 0 (then the pointer may be null).
+ */
+#define MCC_ELEMENT_F32 0
+#define MCC_ELEMENT_F16 1
+#define MCC_ELEMENT_BF16 2
+
+/*
+ * y = (x - mean) * rstd * gain + bias with the row's mean and rstd = 1 / sqrt(variance + eps), the
+ * variance being the mean of the squared differences.  gain and bias (cols floats) may be null: 1 and 0.
+ * mean and rstd (rows floats), which the backward pass needs, may be null.  y may replace x.
+ */
+int mcc_layer_norm(void* stream, const void* x, size_t x_nbytes, size_t x_stride, const float* gain, size_t gain_nbytes,
+                   const float* bias, size_t bias_nbytes, void* y, size_t y_nbytes, size_t y_stride, float* mean,
+                   size_t mean_nbytes, float* rstd, size_t rstd_nbytes, size_t rows, size_t cols, int element, float eps);
+
+/*
+ * Gradients of x, gain and bias for grad_out, the gradient of y, with the mean and rstd of the forward
+ * call.  grad_x, grad_gain and grad_bias may be null (not wanted); gain as in the forward call.  grad_x
+ * may replace grad_out or x.  grad_gain and grad_bias (cols floats) are overwritten with the sums over
+ * all rows.
+ */
+size_t mcc_layer_norm_backward_workspace_nbytes(size_t rows, size_t cols, int element);
+int mcc_layer_norm_backward(void* stream, const void* grad_out, size_t grad_out_nbytes, size_t grad_out_stride,
+                            const void* x, size_t x_nbytes, size_t x_stride, const float* mean, size_t mean_nbytes,
+                            const float* rstd, size_t rstd_nbytes, const float* gain, size_t gain_nbytes, void* grad_x,
+                            size_t grad_x_nbytes, size_t grad_x_stride, float* grad_gain, size_t grad_gain_nbytes,
+                            float* grad_bias, size_t grad_bias_nbytes, void* workspace, size_t workspace_nbytes,
+                            size_t rows, size_t cols, int element);
+
+/*
+ * Of softmax(logits / temperature) for every row of `vocab` logits:
+ *   log_prob       log probability of tokens[row]; 0 where the token is outside [0, vocab) (an ignored
+ *                  position)
+ *   entropy        -sum p log p
+ *   lse            log sum exp(logits / temperature)
+ *   top_ids, top_log_probs [rows, top]   the `top` likeliest tokens, 0 <= top <= MCC_MOST_TOP and <= vocab,
+ *                  with their log probabilities: larger logit first, equal logits (-0 = +0) by the lower
+ *                  token, NaN last
+ * Every output may be null; tokens may be null (then log_prob is 0).  Logits of -inf (masked tokens) have
+ * probability 0 and log probability -inf; in a row of -inf alone every log probability and lse are -inf
+ * and the entropy is 0.  A NaN or +inf makes the row's outputs NaN but for top_ids.
+ */
+#define MCC_MOST_TOP 128
+size_t mcc_token_log_probs_workspace_nbytes(size_t rows, size_t vocab, size_t top, int element);
+int mcc_token_log_probs(void* stream, const void* logits, size_t logits_nbytes, size_t logits_stride,
+                        const int32_t* tokens, size_t tokens_nbytes, float* log_prob, size_t log_prob_nbytes,
+                        float* entropy, size_t entropy_nbytes, float* lse, size_t lse_nbytes, int32_t* top_ids,
+                        size_t top_ids_nbytes, float* top_log_probs, size_t top_log_probs_nbytes, void* workspace,
+                        size_t workspace_nbytes, size_t rows, size_t vocab, size_t top, int element, float temperature);
+
+/*
+ * Gradient of the logits for upstream gradients of log_prob and of entropy (either may be null), from the
+ * forward call's lse and entropy (entropy is looked at only with grad_entropy):
+ *   ((token == j) - p_j) * grad_log_prob - p_j (log p_j + entropy) * grad_entropy,  over temperature.
+ * With grad_log_prob = -1 / n it is the gradient of the mean cross entropy.  Ignored positions take no
+ * grad_log_prob.  Rows whose upstream gradients are zero and rows of -inf alone get zeros whatever their
+ * logits hold.  grad_logits may replace logits.
+ */
+int mcc_token_log_probs_backward(void* stream, const void* logits, size_t logits_nbytes, size_t logits_stride,
+                                 const int32_t* tokens, size_t tokens_nbytes, const float* lse, size_t lse_nbytes,
+                                 const float* entropy, size_t entropy_nbytes, const float* grad_log_prob,
+                                 size_t grad_log_prob_nbytes, const float* grad_entropy, size_t grad_entropy_nbytes,
+                                 void* grad_logits, size_t grad_logits_nbytes, size_t grad_logits_stride, size_t rows,
+                                 size_t vocab, int element, float temperature);
+
+/*
+ * Distillation from a teacher's top logits, such as the top_ids and top_log_probs of
+ * mcc_token_log_probs: with q = softmax(teacher_logits / temperature) over the row's entries and
+ * p = softmax(logits / temperature) over the whole vocabulary,
+ *   loss[row] = temperature^2 * sum q_i (log q_i - log p_id(i)),
+ * and grad_logits = d(sum of weight[row] * loss[row]) / d logits = weight temperature (p_j - sum of the q_i with
+ * id(i) = j).  teacher_ids and teacher_logits are [rows, top], 1 <= top <= MCC_MOST_TOP; an id outside
+ * [0, vocab) is no entry (rows with fewer alternatives), an id may occur more than once.  weight (rows
+ * floats; null: 1), loss and grad_logits may be null; loss is not weighted.  Rows without entries have
+ * loss 0 and gradient 0, rows with weight 0 gradient 0 whatever their logits hold; a row of -inf alone has
+ * loss +inf and gradient 0.  grad_logits may replace logits.
+ */
+size_t mcc_distill_top_workspace_nbytes(size_t rows, size_t vocab, int element);
+int mcc_distill_top(void* stream, const void* logits, size_t logits_nbytes, size_t logits_stride,
+                    const int32_t* teacher_ids, size_t teacher_ids_nbytes, const float* teacher_logits,
+                    size_t teacher_logits_nbytes, const float* weight, size_t weight_nbytes, float* loss,
+                    size_t loss_nbytes, void* grad_logits, size_t grad_logits_nbytes, size_t grad_logits_stride,
+                    void* workspace, size_t workspace_nbytes, size_t rows, size_t vocab, size_t top, int element,
+                    float temperature);
+
+/*
  * Device-resident storage.  Replaces the pooled VulkanRuntime::create_buffer /
  * Storage allocator (src/runtime/vulkan_backend.cpp:4663-4719,6462-6510;
  * src/tensor/storage.cpp:35-79): freed blocks are kept in power-of-two buckets
@@ -385,7 +483,8 @@ int mcc_stream_synchronize(void* stream);
  * bracketed by HIP events on its launch stream; mcc_profiler_query waits for them and
  * returns the summed duration and launch count of one kernel family:
  * "gemm_tn_f32", "counter_update", "counter_decode_weight", "counter_forward",
- * "counter_backward_input".  Replaces Profiler (src/runtime/profiler.cpp) and
+ * "counter_backward_input", "sgd_update", "adam_update", "layer_norm",
+ * "layer_norm_backward", "token_log_probs", "token_log_probs_backward", "distill_top".  Replaces Profiler (src/runtime/profiler.cpp) and
  * VulkanRuntime::set_gpu_timing_enabled / last_gpu_time_us
  * (include/motifcl/runtime/vulkan_backend.hpp:181-185).
  */

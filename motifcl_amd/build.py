@@ -8,7 +8,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmotifcl_amd.so")
 
 SOURCES = ["capi.hip", "counter_update.hip", "gemm_tn_f32.hip", "gemm_tn_f32_wide.hip", "gemm_tn_bf16x6.hip", "counter_fused_strip.hip",
-           "counter_linear.hip", "counter_linear_bf16x3.hip", "side_optim.hip", "diag.hip", "noalloc.hip"]
+           "counter_linear.hip", "counter_linear_bf16x3.hip", "side_optim.hip", "layer_norm.hip", "token_log_probs.hip",
+           "distill_top.hip", "diag.hip", "noalloc.hip"]
 
 # -ffp-contract=off and correctly rounded divide/sqrt make every float operation a single
 # IEEE-754 binary32 rounding, which the bit-exact update relies on.  Packed fp32 ops are
@@ -43,7 +44,7 @@ def build_library(verbose=False, extra_flags=()):
             print(r.stderr)
         return obj
 
-    with ThreadPoolExecutor(max_workers=4) as ex:
+    with ThreadPoolExecutor(max_workers=6) as ex:
         objs = list(ex.map(compile_one, SOURCES))
     cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs]
     r = subprocess.run(cmd, capture_output=True, text=True)

@@ -870,6 +870,237 @@ int mcc_adam_update_f32(void* stream, float* param, size_t param_nbytes, const f
     return MCC_OK;
 }
 
+// ---- row-wise operators --------------------------------------------------------
+namespace {
+
+constexpr size_t kMostColumns = size_t(1) << 30;
+
+bool element_type(int element, mcc::ElementType* type, size_t* size) {
+    switch (element) {
+        case MCC_ELEMENT_F32: *type = mcc::ElementType::F32, *size = 4; return true;
+        case MCC_ELEMENT_F16: *type = mcc::ElementType::F16, *size = 2; return true;
+        case MCC_ELEMENT_BF16: *type = mcc::ElementType::BF16, *size = 2; return true;
+    }
+    return false;
+}
+
+// Rows of elements as an entry point receives them.
+struct RowsArg {
+    const void* p;
+    size_t nbytes, stride;
+};
+// The shape shared by a call's large tensors, and the checks of its buffers; `what` names the operation.
+struct RowsCheck {
+    const char* what;
+    size_t rows, cols;
+    mcc::ElementType type = mcc::ElementType::F32;
+    size_t size = 4;
+
+    bool say(const std::string& message) const {
+        g_error = std::string(what) + " " + message;
+        return false;
+    }
+    bool shape(int element) {
+        if (rows == 0 || cols == 0) return say("requires non-zero dimensions");
+        if (!element_type(element, &type, &size)) return say("received an unknown element type");
+        if (cols > kMostColumns) return say("rows hold at most 2^30 elements");
+        if (rows > kIntMax) return say("rows exceed 2^31-1");
+        return true;
+    }
+    bool tensor(const char* name, const RowsArg& t) const {
+        if (!t.p) return say("received a null buffer");
+        if (reinterpret_cast<uintptr_t>(t.p) % size) return say(std::string(name) + " must be aligned to its elements");
+        if (rows > 1 && t.stride < cols) return say(std::string(name) + " has a stride shorter than its rows");
+        if (rows > 1 && t.stride > (std::numeric_limits<size_t>::max() / size - cols) / (rows - 1))
+            return say(std::string(name) + " size overflows size_t");
+        if (t.nbytes < extent(t)) return say(std::string(name) + " buffer is too small");
+        return true;
+    }
+    // `count` numbers of 4 bytes a row (per_row) or once; null is allowed where `optional`
+    bool numbers(const char* name, const void* p, size_t nbytes, size_t count, bool optional) const {
+        if (!p) return optional || say("received a null buffer");
+        if (reinterpret_cast<uintptr_t>(p) % 4) return say(std::string(name) + " must be 4-byte aligned");
+        if (nbytes < count * 4) return say(std::string(name) + " buffer is too small");
+        return true;
+    }
+    bool workspace(const void* p, size_t nbytes, size_t need) const {
+        if (need == 0) return true;
+        if (!p) return say("received a null buffer");
+        if (reinterpret_cast<uintptr_t>(p) % 16) return say("workspace must be 16-byte aligned");
+        if (nbytes < need) return say("workspace is too small");
+        return true;
+    }
+    size_t extent(const RowsArg& t) const { return ((rows - 1) * (rows > 1 ? t.stride : 0) + cols) * size; }
+    // An output and an input: the same rows, or rows that do not touch (also those that lie between the
+    // other's, as two halves of wider rows do).
+    bool apart(const char* out_name, const RowsArg& out, const char* in_name, const RowsArg& in) const {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(out.p), b = reinterpret_cast<uintptr_t>(in.p);
+        if (a == b && (rows == 1 || out.stride == in.stride)) return true;
+        if (a + extent(out) <= b || b + extent(in) <= a) return true;
+        if (rows > 1 && out.stride == in.stride) {
+            const size_t pitch = out.stride * size, off = (a > b ? a - b : b - a) % pitch;
+            if (off >= cols * size && off + cols * size <= pitch) return true;
+        }
+        return say(std::string(out_name) + " overlaps " + in_name);
+    }
+    bool temperature(float t) const {
+        if (!std::isfinite(t) || !(t > 0.0f) || !std::isfinite(1.0f / t)) return say("requires a positive finite temperature");
+        return true;
+    }
+    // workgroups of one launch
+    bool groups(size_t per_row) const {
+        return rows <= kIntMax / per_row || say("rows times row length exceed what one call takes");
+    }
+};
+
+// Rows are cut into stretches of no less than 4096 elements.
+size_t most_stretches(size_t cols) { return (cols + 4095) / 4096; }
+
+}  // namespace
+
+int mcc_layer_norm(void* stream, const void* x, size_t x_nbytes, size_t x_stride, const float* gain, size_t gain_nbytes,
+                   const float* bias, size_t bias_nbytes, void* y, size_t y_nbytes, size_t y_stride, float* mean,
+                   size_t mean_nbytes, float* rstd, size_t rstd_nbytes, size_t rows, size_t cols, int element, float eps) {
+    RowsCheck c{"layer_norm", rows, cols};
+    const RowsArg xa{x, x_nbytes, x_stride}, ya{y, y_nbytes, y_stride};
+    if (!c.shape(element)) return MCC_E_INVALID;
+    if (!std::isfinite(eps) || eps < 0.0f) return fail(MCC_E_INVALID, "layer_norm requires non-negative finite eps");
+    if (!c.tensor("x", xa) || !c.tensor("y", ya) || !c.apart("y", ya, "x", xa) ||
+        !c.numbers("gain", gain, gain_nbytes, cols, true) || !c.numbers("bias", bias, bias_nbytes, cols, true) ||
+        !c.numbers("mean", mean, mean_nbytes, rows, true) || !c.numbers("rstd", rstd, rstd_nbytes, rows, true))
+        return MCC_E_INVALID;
+    ScopedKernelTimer timer("layer_norm", static_cast<hipStream_t>(stream));
+    const hipError_t e = mcc::launch_layer_norm(static_cast<hipStream_t>(stream), c.type, x, x_stride, gain, bias, y,
+                                                y_stride, mean, rstd, rows, (int)cols, eps);
+    if (e != hipSuccess) return hip_fail(e, "layer_norm launch failed");
+    return MCC_OK;
+}
+
+size_t mcc_layer_norm_backward_workspace_nbytes(size_t rows, size_t cols, int element) {
+    RowsCheck c{"layer_norm_backward", rows, cols};
+    return c.shape(element) ? mcc::layer_norm_backward_workspace_nbytes(c.type, rows, (int)cols) : 0;
+}
+
+int mcc_layer_norm_backward(void* stream, const void* grad_out, size_t grad_out_nbytes, size_t grad_out_stride,
+                            const void* x, size_t x_nbytes, size_t x_stride, const float* mean, size_t mean_nbytes,
+                            const float* rstd, size_t rstd_nbytes, const float* gain, size_t gain_nbytes, void* grad_x,
+                            size_t grad_x_nbytes, size_t grad_x_stride, float* grad_gain, size_t grad_gain_nbytes,
+                            float* grad_bias, size_t grad_bias_nbytes, void* workspace, size_t workspace_nbytes,
+                            size_t rows, size_t cols, int element) {
+    RowsCheck c{"layer_norm_backward", rows, cols};
+    const RowsArg da{grad_out, grad_out_nbytes, grad_out_stride}, xa{x, x_nbytes, x_stride},
+        ga{grad_x, grad_x_nbytes, grad_x_stride};
+    if (!c.shape(element) || !c.tensor("grad_out", da) || !c.tensor("x", xa) ||
+        !c.numbers("mean", mean, mean_nbytes, rows, false) || !c.numbers("rstd", rstd, rstd_nbytes, rows, false) ||
+        !c.numbers("gain", gain, gain_nbytes, cols, true) || !c.numbers("grad_gain", grad_gain, grad_gain_nbytes, cols, true) ||
+        !c.numbers("grad_bias", grad_bias, grad_bias_nbytes, cols, true))
+        return MCC_E_INVALID;
+    if (grad_x && (!c.tensor("grad_x", ga) || !c.apart("grad_x", ga, "grad_out", da) || !c.apart("grad_x", ga, "x", xa)))
+        return MCC_E_INVALID;
+    if (!grad_x && !grad_gain && !grad_bias) return fail(MCC_E_INVALID, "layer_norm_backward received no output");
+    if ((grad_gain || grad_bias) &&
+        !c.workspace(workspace, workspace_nbytes, mcc::layer_norm_backward_workspace_nbytes(c.type, rows, (int)cols)))
+        return MCC_E_INVALID;
+    ScopedKernelTimer timer("layer_norm_backward", static_cast<hipStream_t>(stream));
+    const hipError_t e = mcc::launch_layer_norm_backward(static_cast<hipStream_t>(stream), c.type, grad_out, grad_out_stride,
+                                                         x, x_stride, mean, rstd, gain, grad_x, grad_x_stride, grad_gain,
+                                                         grad_bias, static_cast<float*>(workspace), rows, (int)cols);
+    if (e != hipSuccess) return hip_fail(e, "layer_norm_backward launch failed");
+    return MCC_OK;
+}
+
+size_t mcc_token_log_probs_workspace_nbytes(size_t rows, size_t vocab, size_t top, int element) {
+    RowsCheck c{"token_log_probs", rows, vocab};
+    if (!c.shape(element) || top > MCC_MOST_TOP || top > vocab || !c.groups(most_stretches(vocab))) return 0;
+    return mcc::token_log_probs_workspace_nbytes(c.type, rows, (int)vocab, (int)top);
+}
+
+int mcc_token_log_probs(void* stream, const void* logits, size_t logits_nbytes, size_t logits_stride,
+                        const int32_t* tokens, size_t tokens_nbytes, float* log_prob, size_t log_prob_nbytes,
+                        float* entropy, size_t entropy_nbytes, float* lse, size_t lse_nbytes, int32_t* top_ids,
+                        size_t top_ids_nbytes, float* top_log_probs, size_t top_log_probs_nbytes, void* workspace,
+                        size_t workspace_nbytes, size_t rows, size_t vocab, size_t top, int element, float temperature) {
+    RowsCheck c{"token_log_probs", rows, vocab};
+    if (!c.shape(element) || !c.temperature(temperature)) return MCC_E_INVALID;
+    if (top > MCC_MOST_TOP || top > vocab)
+        return fail(MCC_E_INVALID, "token_log_probs gives at most 128 and at most vocab alternatives");
+    if (!c.tensor("logits", {logits, logits_nbytes, logits_stride}) || !c.groups(most_stretches(vocab)) ||
+        !c.numbers("tokens", tokens, tokens_nbytes, rows, true) ||
+        !c.numbers("log_prob", log_prob, log_prob_nbytes, rows, true) ||
+        !c.numbers("entropy", entropy, entropy_nbytes, rows, true) || !c.numbers("lse", lse, lse_nbytes, rows, true) ||
+        !c.numbers("top_ids", top_ids, top_ids_nbytes, rows * top, true) ||
+        !c.numbers("top_log_probs", top_log_probs, top_log_probs_nbytes, rows * top, true) ||
+        !c.workspace(workspace, workspace_nbytes, mcc::token_log_probs_workspace_nbytes(c.type, rows, (int)vocab, (int)top)))
+        return MCC_E_INVALID;
+    const mcc::TokenLogProbs a{logits, logits_stride, rows, (int)vocab, (int)top, 1.0f / temperature, tokens,
+                               log_prob, entropy, lse, top_ids, top_log_probs};
+    ScopedKernelTimer timer("token_log_probs", static_cast<hipStream_t>(stream));
+    const hipError_t e = mcc::launch_token_log_probs(static_cast<hipStream_t>(stream), c.type, a, workspace);
+    if (e != hipSuccess) return hip_fail(e, "token_log_probs launch failed");
+    return MCC_OK;
+}
+
+int mcc_token_log_probs_backward(void* stream, const void* logits, size_t logits_nbytes, size_t logits_stride,
+                                 const int32_t* tokens, size_t tokens_nbytes, const float* lse, size_t lse_nbytes,
+                                 const float* entropy, size_t entropy_nbytes, const float* grad_log_prob,
+                                 size_t grad_log_prob_nbytes, const float* grad_entropy, size_t grad_entropy_nbytes,
+                                 void* grad_logits, size_t grad_logits_nbytes, size_t grad_logits_stride, size_t rows,
+                                 size_t vocab, int element, float temperature) {
+    RowsCheck c{"token_log_probs_backward", rows, vocab};
+    const RowsArg la{logits, logits_nbytes, logits_stride}, ga{grad_logits, grad_logits_nbytes, grad_logits_stride};
+    if (!c.shape(element) || !c.temperature(temperature) || !c.groups(most_stretches(vocab)) || !c.tensor("logits", la) ||
+        !c.tensor("grad_logits", ga) || !c.apart("grad_logits", ga, "logits", la) ||
+        !c.numbers("tokens", tokens, tokens_nbytes, rows, !grad_log_prob) || !c.numbers("lse", lse, lse_nbytes, rows, false) ||
+        !c.numbers("entropy", entropy, entropy_nbytes, rows, !grad_entropy) ||
+        !c.numbers("grad_log_prob", grad_log_prob, grad_log_prob_nbytes, rows, true) ||
+        !c.numbers("grad_entropy", grad_entropy, grad_entropy_nbytes, rows, true))
+        return MCC_E_INVALID;
+    if (!grad_log_prob && !grad_entropy)
+        return fail(MCC_E_INVALID, "token_log_probs_backward received no upstream gradient");
+    ScopedKernelTimer timer("token_log_probs_backward", static_cast<hipStream_t>(stream));
+    const hipError_t e = mcc::launch_token_log_probs_backward(static_cast<hipStream_t>(stream), c.type, logits,
+                                                              logits_stride, tokens, lse, entropy, grad_log_prob,
+                                                              grad_entropy, grad_logits, grad_logits_stride, rows,
+                                                              (int)vocab, 1.0f / temperature);
+    if (e != hipSuccess) return hip_fail(e, "token_log_probs_backward launch failed");
+    return MCC_OK;
+}
+
+size_t mcc_distill_top_workspace_nbytes(size_t rows, size_t vocab, int element) {
+    RowsCheck c{"distill_top", rows, vocab};
+    if (!c.shape(element) || !c.groups(most_stretches(vocab))) return 0;
+    return mcc::distill_top_workspace_nbytes(c.type, rows, (int)vocab);
+}
+
+int mcc_distill_top(void* stream, const void* logits, size_t logits_nbytes, size_t logits_stride,
+                    const int32_t* teacher_ids, size_t teacher_ids_nbytes, const float* teacher_logits,
+                    size_t teacher_logits_nbytes, const float* weight, size_t weight_nbytes, float* loss,
+                    size_t loss_nbytes, void* grad_logits, size_t grad_logits_nbytes, size_t grad_logits_stride,
+                    void* workspace, size_t workspace_nbytes, size_t rows, size_t vocab, size_t top, int element,
+                    float temperature) {
+    RowsCheck c{"distill_top", rows, vocab};
+    const RowsArg la{logits, logits_nbytes, logits_stride}, ga{grad_logits, grad_logits_nbytes, grad_logits_stride};
+    if (!c.shape(element) || !c.temperature(temperature)) return MCC_E_INVALID;
+    if (top == 0 || top > MCC_MOST_TOP) return fail(MCC_E_INVALID, "distill_top takes 1 to 128 of a teacher's logits a row");
+    if (!std::isfinite(temperature * temperature))
+        return fail(MCC_E_INVALID, "distill_top requires a temperature whose square is finite");
+    if (!c.groups(most_stretches(vocab)) || !c.tensor("logits", la) ||
+        !c.numbers("teacher_ids", teacher_ids, teacher_ids_nbytes, rows * top, false) ||
+        !c.numbers("teacher_logits", teacher_logits, teacher_logits_nbytes, rows * top, false) ||
+        !c.numbers("weight", weight, weight_nbytes, rows, true) || !c.numbers("loss", loss, loss_nbytes, rows, true))
+        return MCC_E_INVALID;
+    if (grad_logits && (!c.tensor("grad_logits", ga) || !c.apart("grad_logits", ga, "logits", la))) return MCC_E_INVALID;
+    if (!loss && !grad_logits) return fail(MCC_E_INVALID, "distill_top received no output");
+    if (!c.workspace(workspace, workspace_nbytes, mcc::distill_top_workspace_nbytes(c.type, rows, (int)vocab)))
+        return MCC_E_INVALID;
+    const mcc::DistillTop a{logits, logits_stride, rows, (int)vocab, (int)top, temperature, 1.0f / temperature,
+                            teacher_ids, teacher_logits, weight, loss, grad_logits, grad_logits_stride};
+    ScopedKernelTimer timer("distill_top", static_cast<hipStream_t>(stream));
+    const hipError_t e = mcc::launch_distill_top(static_cast<hipStream_t>(stream), c.type, a, workspace);
+    if (e != hipSuccess) return hip_fail(e, "distill_top launch failed");
+    return MCC_OK;
+}
+
 int mcc_memset_zero(void* stream, void* dst, size_t nbytes) {
     if (nbytes == 0) return MCC_OK;
     if (!dst) return fail(MCC_E_INVALID, "memset received a null pointer");

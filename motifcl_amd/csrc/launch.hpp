@@ -149,4 +149,58 @@ hipError_t launch_adam_update(hipStream_t stream, float* param, const float* gra
                               size_t n, float lr, float beta1, float beta2, float eps, float inv_bias1,
                               float inv_bias2, float weight_decay);
 
+// ---- row-wise operators --------------------------------------------------------------------------
+// Strides are elements between the starts of two rows; rows and lengths are at least 1.
+enum class ElementType { F32, F16, BF16 };
+
+// y = (x - mean) * rstd * gain + bias (layer_norm.hip); gain, bias, mean and rstd may be null, y may
+// be x with the same stride.
+hipError_t launch_layer_norm(hipStream_t stream, ElementType type, const void* x, size_t x_stride, const float* gain,
+                             const float* bias, void* y, size_t y_stride, float* mean, float* rstd, size_t rows, int n,
+                             float eps);
+// The gradients of x, gain and bias; each of the three may be null.  The workspace holds the partial
+// sums of the two column gradients.
+size_t layer_norm_backward_workspace_nbytes(ElementType type, size_t rows, int n);
+hipError_t launch_layer_norm_backward(hipStream_t stream, ElementType type, const void* grad_out, size_t grad_out_stride,
+                                      const void* x, size_t x_stride, const float* mean, const float* rstd,
+                                      const float* gain, void* grad_x, size_t grad_x_stride, float* grad_gain,
+                                      float* grad_bias, float* workspace, size_t rows, int n);
+
+// The `top` likeliest entries, the entropy and the given token's log probability of softmax(logits /
+// temperature) (token_log_probs.hip); every output may be null, `top` at most kMostTop.
+constexpr int kMostTop = 128;
+struct TokenLogProbs {
+    const void* logits;
+    size_t stride, rows;
+    int vocab, top;
+    float inv_temperature;
+    const int32_t* tokens;
+    float *log_prob, *entropy, *lse;
+    int32_t* top_ids;
+    float* top_log_probs;
+};
+size_t token_log_probs_workspace_nbytes(ElementType type, size_t rows, int vocab, int top);
+hipError_t launch_token_log_probs(hipStream_t stream, ElementType type, const TokenLogProbs& a, void* workspace);
+hipError_t launch_token_log_probs_backward(hipStream_t stream, ElementType type, const void* logits, size_t stride,
+                                           const int32_t* tokens, const float* lse, const float* entropy,
+                                           const float* grad_log_prob, const float* grad_entropy, void* grad_logits,
+                                           size_t grad_stride, size_t rows, int vocab, float inv_temperature);
+
+// temperature^2 * KL(teacher || student) over the teacher's `top` entries, and the gradient of the
+// weighted sum of the rows' losses (distill_top.hip); weight, loss and grad may be null.
+struct DistillTop {
+    const void* logits;
+    size_t stride, rows;
+    int vocab, top;
+    float temperature, inv_temperature;
+    const int32_t* ids;      // [rows, top], outside [0, vocab): no entry
+    const float* teacher;    // [rows, top]
+    const float* weight;     // [rows]
+    float* loss;             // [rows]
+    void* grad;
+    size_t grad_stride;
+};
+size_t distill_top_workspace_nbytes(ElementType type, size_t rows, int vocab);
+hipError_t launch_distill_top(hipStream_t stream, ElementType type, const DistillTop& a, void* workspace);
+
 }  // namespace mcc

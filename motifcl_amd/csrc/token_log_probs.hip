@@ -1,0 +1,474 @@
+// Log probabilities of given tokens under softmax(logits / temperature), the entropy of that
+// distribution, its `top` likeliest tokens, and the gradient of the logits.
+//     log p_j = (z_j - m) / T - log s,  H = log s - u / s               (row_softmax.hpp)
+//     dz_j = (g (delta_j,token - p_j) - h p_j (log p_j + H)) / T        for upstream gradients g of log p and h of H
+// Bound by memory: the logits are read once, into registers, by one workgroup a row or, where rows are
+// long or few, by one a stretch of a row; a second launch then joins the stretches.  The top entries are
+// found in the registers: numbers below a bound that at least `top` numbers reach are passed over, and
+// the few that are left are ranked.  Order: larger logit first, among equals the lower token, -0 = +0,
+// NaN behind -inf; so equal calls give equal bytes whatever order the candidates were found in.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+
+#include "launch.hpp"
+#include "row_softmax.hpp"
+#include "row_values.hpp"
+
+namespace mcc {
+namespace {
+
+constexpr uint32_t kKeyLowest = 0x007fffffu;   // key of -inf
+constexpr uint32_t kKeyHighest = 0xff800000u;  // key of +inf
+
+// Unsigned integers in the order of the floats they stand for.
+__device__ __forceinline__ uint32_t key_of(float z) {
+    if (!(z == z)) return 0;
+    const uint32_t b = __float_as_uint(z + 0.0f);  // -0 becomes +0
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float of_key(uint32_t k) {
+    if (k == 0) return __uint_as_float(0x7fc00000u);
+    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+// A candidate: larger is likelier, and among equal logits the lower token is larger.
+__device__ __forceinline__ uint64_t candidate(float z, uint32_t id) { return (uint64_t)key_of(z) << 32 | (uint32_t)~id; }
+
+constexpr int kCandidates = 512;
+template <int WAVES>
+struct TopScratch {
+    uint64_t list[kCandidates];
+    uint32_t bound[WAVES];
+    int count;
+    int totals[2][WAVES];
+};
+
+// Sum over the workgroup of a count per wave; `turn` alternates between calls.
+template <int WAVES>
+__device__ __forceinline__ int total_of(int wave_count, int (&totals)[2][WAVES], int turn, int wave, int lane) {
+    if (WAVES == 1) return wave_count;
+    if (lane == 0) totals[turn][wave] = wave_count;
+    __syncthreads();
+    int a = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) a += totals[turn][w];
+    return a;
+}
+
+// A number that at least `top` of the workgroup's numbers reach, as a float: every wave gives the
+// ceil(top / WAVES)-th largest of its lanes' maxima (rounded down to a multiple of 64 units of the key,
+// which makes room for the lane), and the smallest of those is reached by as many lanes of every wave.
+template <int WAVES>
+__device__ __forceinline__ float lower_bound_of(float thread_max, int top, TopScratch<WAVES>& lds, int wave, int lane) {
+    const int nth = (top + WAVES - 1) / WAVES;
+    const uint32_t mine = (key_of(thread_max) & ~63u) | (uint32_t)(63 - lane);
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < 64; ++i) above += (uint32_t)__builtin_amdgcn_readlane((int)mine, i) > mine ? 1 : 0;
+    uint32_t bound = 0;
+    if (nth <= 64) {
+        const uint64_t there = __builtin_amdgcn_ballot_w64(above == nth - 1);
+        bound = (uint32_t)__builtin_amdgcn_readlane((int)mine, __builtin_ctzll(there)) & ~63u;
+    }
+    if (WAVES > 1) {
+        if (lane == 0) lds.bound[wave] = bound;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) bound = lds.bound[w] < bound ? lds.bound[w] : bound;
+    }
+    return bound <= kKeyLowest ? -__builtin_inff() : of_key(bound);
+}
+
+// The `top` candidates of a stretch into lds.list[0 .. top) when too many numbers (ties, as of masked
+// logits) reach the bound, or too few (NaN): the top-th largest key by bisection over its bits, the
+// numbers above it, and the first of those equal to it.
+template <typename ROW, int WAVES, int ITERS>
+__device__ __forceinline__ void select_by_bisection(const ROW& r, int n, uint32_t first_id, int top, TopScratch<WAVES>& lds,
+                                                 int t, int wave, int lane) {
+    int turn = 0;
+    auto count = [&](auto test) {
+        int c = 0;
+#pragma unroll
+        for (int j = 0; j < ITERS; ++j)
+#pragma unroll
+            for (int k = 0; k < ROW::kVec; ++k) c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(test(j, k)));
+        turn ^= 1;
+        return total_of<WAVES>(c, lds.totals, turn, wave, lane);
+    };
+    auto value = [&](int j, int k) { return (float)r.raw[j][k]; };
+    const int numbers = count([&](int j, int k) { return value(j, k) >= -__builtin_inff() && ROW::holds(j, k, t, n); });
+    uint32_t key = 0;
+    if (numbers >= top) {
+#pragma unroll 1
+        for (int bit = 31; bit >= 0; --bit) {
+            const uint32_t next = key | 1u << bit;
+            if (next > kKeyHighest) continue;
+            if (next > kKeyLowest) {  // at least `top` numbers reach -inf; above it the filled ones do not count
+                const float f = of_key(next);
+                if (count([&](int j, int k) { return value(j, k) >= f; }) < top) continue;
+            }
+            key = next;
+        }
+    }
+    const float f = key ? of_key(key) : 0.0f;
+    // key 0: all numbers are above, and NaN are the ties
+    auto above = [&](int j, int k) { return key ? value(j, k) > f : value(j, k) >= -__builtin_inff() && ROW::holds(j, k, t, n); };
+    auto equal = [&](int j, int k) { return (key ? value(j, k) == f : !(value(j, k) == value(j, k))) && ROW::holds(j, k, t, n); };
+    const int n_above = count(above);
+    __syncthreads();
+    if (t == 0) lds.count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ITERS; ++j)
+#pragma unroll
+        for (int k = 0; k < ROW::kVec; ++k)
+            if (above(j, k)) {
+                const int at = atomicAdd(&lds.count, 1);
+                if (at < kCandidates) lds.list[at] = candidate(value(j, k), first_id + ROW::index(j, k, t, n));
+            }
+    // ties in the order of their tokens: vector by vector, in it thread by thread
+    int before = n_above;
+#pragma unroll
+    for (int j = 0; j < ITERS; ++j) {
+        int of_wave = 0, lower = 0;
+        const uint64_t below = ((uint64_t)1 << lane) - 1;
+#pragma unroll
+        for (int k = 0; k < ROW::kVec; ++k) {
+            const uint64_t b = __builtin_amdgcn_ballot_w64(equal(j, k));
+            of_wave += __builtin_popcountll(b);
+            lower += __builtin_popcountll(b & below);
+        }
+        turn ^= 1;
+        const int all = total_of<WAVES>(of_wave, lds.totals, turn, wave, lane);
+        int at = before + lower;
+        for (int w = 0; w < wave; ++w) at += lds.totals[turn][w];
+#pragma unroll
+        for (int k = 0; k < ROW::kVec; ++k)
+            if (equal(j, k)) {
+                if (at < top) lds.list[at] = candidate(value(j, k), first_id + ROW::index(j, k, t, n));
+                ++at;
+            }
+        before += all;
+    }
+    __syncthreads();
+}
+
+// The candidates of a stretch, unordered, in lds.list; returns their number (at least `top`, at most
+// kCandidates).  n >= top.
+template <typename ROW, int WAVES, int ITERS>
+__device__ __forceinline__ int find_candidates(const ROW& r, int n, uint32_t first_id, int top, float thread_max,
+                                               TopScratch<WAVES>& lds, int t, int wave, int lane) {
+    if (t == 0) lds.count = 0;
+    const float bound = lower_bound_of<WAVES>(thread_max, top, lds, wave, lane);
+    if (WAVES == 1) __syncthreads();
+    if (thread_max >= bound) {
+#pragma unroll
+        for (int j = 0; j < ITERS; ++j)
+#pragma unroll
+            for (int k = 0; k < ROW::kVec; ++k) {
+                const float z = (float)r.raw[j][k];
+                if (z >= bound && ROW::holds(j, k, t, n)) {
+                    const int at = atomicAdd(&lds.count, 1);
+                    if (at < kCandidates) lds.list[at] = candidate(z, first_id + ROW::index(j, k, t, n));
+                }
+            }
+    }
+    __syncthreads();
+    const int found = lds.count;
+    if (found >= top && found <= kCandidates) return found;
+    select_by_bisection<ROW, WAVES, ITERS>(r, n, first_id, top, lds, t, wave, lane);
+    return top;
+}
+
+// What is left of a row's statistics once they are joined.
+struct RowResult {
+    float m, log_s, inv_temperature;
+    bool empty;  // -inf alone
+    __device__ __forceinline__ float log_prob(float z) const {
+        return empty && z == z ? -__builtin_inff() : (z - m) * inv_temperature - log_s;
+    }
+};
+__device__ __forceinline__ RowResult finish_row(const TokenLogProbs& a, size_t row, const SoftmaxStats& st, float token_logit,
+                                                bool has_token, bool writes) {
+    RowResult r;
+    r.m = st.m;
+    r.empty = st.s == 0.0f;
+    r.log_s = logf(st.s);
+    r.inv_temperature = a.inv_temperature;
+    if (writes) {
+        if (a.lse) a.lse[row] = r.empty ? -__builtin_inff() : st.m * a.inv_temperature + r.log_s;
+        if (a.entropy) a.entropy[row] = r.empty ? 0.0f : r.log_s - st.u / st.s;
+        if (a.log_prob) a.log_prob[row] = has_token ? r.log_prob(token_logit) : 0.0f;
+    }
+    return r;
+}
+
+template <typename T>
+__device__ __forceinline__ bool token_of(const TokenLogProbs& a, size_t row, float& z) {
+    if (!a.tokens || !a.log_prob) return false;
+    const int32_t token = a.tokens[row];
+    if (token < 0 || token >= a.vocab) return false;  // an ignored position
+    z = (float)static_cast<const T*>(a.logits)[row * a.stride + token];
+    return true;
+}
+
+// One stretch a workgroup.  ONE: the row is one stretch, and the results are written; else `stats` and
+// `best` [rows * segments][top] are.
+template <typename T, int THREADS, int PER_THREAD, bool TOP, bool ONE>
+__global__ __launch_bounds__(THREADS) void token_log_probs_kernel(TokenLogProbs a, int segments, int length,
+                                                                  SoftmaxStats* stats, uint64_t* best) {
+    constexpr int kIters = PER_THREAD / Elements<T>::kVec, kWaves = THREADS / 64;
+    typedef RowVectors<T, THREADS, kIters> Row;
+    __shared__ float slots[3 * kWaves];
+    __shared__ TopScratch<TOP ? kWaves : 1> lds;
+    const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
+    const size_t row = ONE ? blockIdx.x : blockIdx.x / (unsigned)segments;
+    const int segment = ONE ? 0 : (int)(blockIdx.x % (unsigned)segments);
+    const int from = segment * length, n = a.vocab - from < length ? a.vocab - from : length;
+    Row r;
+    r.load(static_cast<const T*>(a.logits) + row * a.stride + from, t, n);
+    float token_logit = 0.0f;
+    const bool has_token = ONE && t == 0 && token_of<T>(a, row, token_logit);
+    r.fill_tail(t, n, (T)-__builtin_inff());
+    float thread_max;
+    const SoftmaxStats st = stats_of<Row, kWaves, kIters>(r, a.inv_temperature, slots, wave, lane, thread_max);
+    RowResult result{};
+    if (ONE)
+        result = finish_row(a, row, st, token_logit, has_token, t == 0);
+    else if (t == 0)
+        stats[row * segments + segment] = st;
+    if constexpr (TOP) {
+        const int top = a.top < n ? a.top : n;
+        const int found = find_candidates<Row, kWaves, kIters>(r, n, (uint32_t)from, top, thread_max, lds, t, wave, lane);
+        for (int i = t; i < found; i += THREADS) {
+            const uint64_t mine = lds.list[i];
+            int rank = 0;
+            for (int k = 0; k < found; ++k) rank += lds.list[k] > mine ? 1 : 0;
+            if (rank >= top) continue;
+            if (ONE) {
+                if (a.top_ids) a.top_ids[row * a.top + rank] = (int32_t)~(uint32_t)mine;
+                if (a.top_log_probs) a.top_log_probs[row * a.top + rank] = result.log_prob(of_key((uint32_t)(mine >> 32)));
+            } else {
+                best[(row * segments + segment) * a.top + rank] = mine;
+            }
+        }
+        if (!ONE)
+            for (int i = top + t; i < a.top; i += THREADS) best[(row * segments + segment) * a.top + i] = 0;
+    }
+}
+
+// Joins a row's stretches.  The entries that reach the smallest of the stretches' ceil(top / segments)-th
+// ones (at least `top` do) are ranked; where they are too many, as when one stretch holds most of the
+// likely tokens, the top-th largest is found by bisection first.
+constexpr int kJoinThreads = 256, kJoinCandidates = 1024;
+template <typename T>
+__global__ __launch_bounds__(kJoinThreads) void token_log_probs_join_kernel(TokenLogProbs a, int segments,
+                                                                           const SoftmaxStats* stats,
+                                                                           const uint64_t* best) {
+    constexpr int kWaves = kJoinThreads / 64;
+    __shared__ uint64_t list[kJoinCandidates];
+    __shared__ int count, totals[2][kWaves];
+    __shared__ uint64_t bounds[kWaves];
+    const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
+    const size_t row = blockIdx.x;
+    float token_logit = 0.0f;
+    const bool has_token = t == 0 && token_of<T>(a, row, token_logit);
+    SoftmaxStats st = stats[row * segments];
+    for (int i = 1; i < segments; ++i) st = join_stats(st, stats[row * segments + i], a.inv_temperature);
+    const RowResult result = finish_row(a, row, st, token_logit, has_token, t == 0);
+    if (a.top == 0 || (!a.top_ids && !a.top_log_probs)) return;
+    const uint64_t* entries = best + row * segments * a.top;
+    const int all = segments * a.top, nth = (a.top + segments - 1) / segments;
+    uint64_t bound = ~(uint64_t)0;
+    for (int i = t; i < segments; i += kJoinThreads) {
+        const uint64_t e = entries[i * a.top + nth - 1];
+        bound = e < bound ? e : bound;
+    }
+    for (int s = 32; s >= 1; s >>= 1) {
+        const uint64_t e = __shfl_xor(bound, s);
+        bound = e < bound ? e : bound;
+    }
+    if (lane == 0) bounds[wave] = bound;
+    if (t == 0) count = 0;
+    __syncthreads();
+    for (int w = 0; w < kWaves; ++w) bound = bounds[w] < bound ? bounds[w] : bound;
+    auto gather = [&](uint64_t from) {
+        for (int i = t; i < all; i += kJoinThreads) {
+            const uint64_t e = entries[i];
+            if (e >= from && e != 0) {  // 0: a stretch shorter than `top` has no such entry
+                const int at = atomicAdd(&count, 1);
+                if (at < kJoinCandidates) list[at] = e;
+            }
+        }
+        __syncthreads();
+    };
+    gather(bound);
+    int found = count;
+    if (found > kJoinCandidates) {
+        uint64_t kth = 0;
+        int turn = 0;
+        for (int bit = 63; bit >= 0; --bit) {
+            const uint64_t next = kth | (uint64_t)1 << bit;
+            int c = 0;
+            for (int i = t; i < (all + 63) / 64 * 64; i += kJoinThreads)
+                c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(i < all && entries[i] >= next));
+            turn ^= 1;
+            if (total_of<kWaves>(c, totals, turn, wave, lane) >= a.top) kth = next;
+        }
+        __syncthreads();
+        if (t == 0) count = 0;
+        __syncthreads();
+        gather(kth);
+        found = count;
+    }
+    for (int i = t; i < found; i += kJoinThreads) {
+        const uint64_t mine = list[i];
+        int rank = 0;
+        for (int k = 0; k < found; ++k) rank += list[k] > mine ? 1 : 0;
+        if (rank >= a.top) continue;
+        if (a.top_ids) a.top_ids[row * a.top + rank] = (int32_t)~(uint32_t)mine;
+        if (a.top_log_probs) a.top_log_probs[row * a.top + rank] = result.log_prob(of_key((uint32_t)(mine >> 32)));
+    }
+}
+
+// ---- backward -----------------------------------------------------------------------------------
+// A stream of logits in and gradients out; the row's numbers are known beforehand.  grad_logits may be
+// logits (one thread owns an element).
+constexpr int kGradThreads = 256, kGradPerThread = 16;
+template <typename T, bool ENTROPY>
+__global__ __launch_bounds__(kGradThreads) void token_log_probs_backward_kernel(
+    const T* logits, size_t stride, const int32_t* tokens, const float* lse, const float* entropy,
+    const float* grad_log_prob, const float* grad_entropy, T* grad_logits, size_t grad_stride, int segments, int vocab,
+    float inv_temperature) {
+    constexpr int kIters = kGradPerThread / Elements<T>::kVec, kLength = kGradThreads * kGradPerThread;
+    typedef RowVectors<T, kGradThreads, kIters> Row;
+    const int t = threadIdx.x;
+    const size_t row = blockIdx.x / (unsigned)segments;
+    const int from = (int)(blockIdx.x % (unsigned)segments) * kLength;
+    const int n = vocab - from < kLength ? vocab - from : kLength;
+    Row r;
+    r.load(logits + row * stride + from, t, n);
+    const int32_t token = tokens ? tokens[row] : -1;
+    const float l = lse[row], big_h = ENTROPY ? entropy[row] : 0.0f;
+    const float g = grad_log_prob && token >= 0 && token < vocab ? grad_log_prob[row] : 0.0f;
+    const float h = ENTROPY ? grad_entropy[row] : 0.0f;
+    // nothing upstream, or a row of -inf alone: zeros, whatever the logits hold
+    const bool zero = (g == 0.0f && h == 0.0f) || l == -__builtin_inff();
+#pragma unroll
+    for (int j = 0; j < kIters; ++j) {
+        float v[Row::kVec];
+#pragma unroll
+        for (int k = 0; k < Row::kVec; ++k) {
+            const float log_p = (float)r.raw[j][k] * inv_temperature - l, p = fast_exp(log_p);
+            float q = -g * p;
+            if (ENTROPY) q -= h * (p * (fmaxf(log_p, -1e4f) + big_h));  // p is 0 long before the bound
+            if (from + Row::index(j, k, t, n) == token) q += g;
+            v[k] = zero ? 0.0f : q * inv_temperature;
+        }
+        store_row_vector<T, kGradThreads, kIters>(grad_logits + row * grad_stride + from, j, t, n, v);
+    }
+}
+
+// Workspace of a row cut into stretches: their statistics, then their entries.
+size_t stats_nbytes(size_t rows, const RowCut& c) { return (rows * c.segments * sizeof(SoftmaxStats) + 15) / 16 * 16; }
+
+template <typename T, bool TOP, bool ONE>
+hipError_t launch_stretches(hipStream_t stream, const TokenLogProbs& a, const RowCut& c, SoftmaxStats* stats, uint64_t* best) {
+    const dim3 grid((unsigned)(a.rows * c.segments));
+#define MCC_STRETCH(THREADS, PER_THREAD)                                                                             \
+    if (c.threads == THREADS && c.per_thread == PER_THREAD)                                                          \
+    hipLaunchKernelGGL((token_log_probs_kernel<T, THREADS, PER_THREAD, TOP, ONE>), grid, dim3(THREADS), 0, stream, a, \
+                       c.segments, c.length, stats, best)
+    MCC_STRETCH(64, 8);
+    MCC_STRETCH(64, 32);
+    MCC_STRETCH(256, 16);
+    MCC_STRETCH(256, 32);
+    MCC_STRETCH(512, 32);
+    MCC_STRETCH(1024, 32);
+#undef MCC_STRETCH
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t forward(hipStream_t stream, const TokenLogProbs& a, void* workspace) {
+    const RowCut c = cut_rows(a.rows, a.vocab);
+    const bool top = a.top > 0 && (a.top_ids || a.top_log_probs);
+    if (c.segments == 1)
+        return top ? launch_stretches<T, true, true>(stream, a, c, nullptr, nullptr)
+                   : launch_stretches<T, false, true>(stream, a, c, nullptr, nullptr);
+    SoftmaxStats* stats = static_cast<SoftmaxStats*>(workspace);
+    uint64_t* best = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + stats_nbytes(a.rows, c));
+    const hipError_t e = top ? launch_stretches<T, true, false>(stream, a, c, stats, best)
+                             : launch_stretches<T, false, false>(stream, a, c, stats, best);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(token_log_probs_join_kernel<T>, dim3((unsigned)a.rows), dim3(kJoinThreads), 0, stream, a, c.segments,
+                       stats, best);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t backward(hipStream_t stream, const void* logits, size_t stride, const int32_t* tokens, const float* lse,
+                    const float* entropy, const float* grad_log_prob, const float* grad_entropy, void* grad_logits,
+                    size_t grad_stride, size_t rows, int vocab, float inv_temperature) {
+    constexpr int length = kGradThreads * kGradPerThread;
+    const int segments = (int)(((size_t)vocab + length - 1) / length);
+    const dim3 grid((unsigned)(rows * segments)), block(kGradThreads);
+    if (grad_entropy)
+        hipLaunchKernelGGL((token_log_probs_backward_kernel<T, true>), grid, block, 0, stream, static_cast<const T*>(logits),
+                           stride, tokens, lse, entropy, grad_log_prob, grad_entropy, static_cast<T*>(grad_logits),
+                           grad_stride, segments, vocab, inv_temperature);
+    else
+        hipLaunchKernelGGL((token_log_probs_backward_kernel<T, false>), grid, block, 0, stream,
+                           static_cast<const T*>(logits), stride, tokens, lse, entropy, grad_log_prob, grad_entropy,
+                           static_cast<T*>(grad_logits), grad_stride, segments, vocab, inv_temperature);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+size_t token_log_probs_workspace_nbytes(ElementType, size_t rows, int vocab, int top) {
+    const RowCut c = cut_rows(rows, vocab);
+    if (c.segments == 1) return 0;
+    return stats_nbytes(rows, c) + rows * c.segments * (size_t)top * sizeof(uint64_t);
+}
+
+hipError_t launch_token_log_probs(hipStream_t stream, ElementType type, const TokenLogProbs& a, void* workspace) {
+    switch (type) {
+        case ElementType::F32: return forward<float>(stream, a, workspace);
+        case ElementType::F16: return forward<_Float16>(stream, a, workspace);
+        case ElementType::BF16: return forward<__bf16>(stream, a, workspace);
+    }
+    return hipErrorInvalidValue;
+}
+
+hipError_t launch_softmax_stats(hipStream_t stream, ElementType type, const void* logits, size_t stride, size_t rows,
+                                int vocab, float inv_temperature, const RowCut& cut, SoftmaxStats* stats) {
+    TokenLogProbs a{};
+    a.logits = logits, a.stride = stride, a.rows = rows, a.vocab = vocab, a.inv_temperature = inv_temperature;
+    switch (type) {
+        case ElementType::F32: return launch_stretches<float, false, false>(stream, a, cut, stats, nullptr);
+        case ElementType::F16: return launch_stretches<_Float16, false, false>(stream, a, cut, stats, nullptr);
+        case ElementType::BF16: return launch_stretches<__bf16, false, false>(stream, a, cut, stats, nullptr);
+    }
+    return hipErrorInvalidValue;
+}
+
+hipError_t launch_token_log_probs_backward(hipStream_t stream, ElementType type, const void* logits, size_t stride,
+                                           const int32_t* tokens, const float* lse, const float* entropy,
+                                           const float* grad_log_prob, const float* grad_entropy, void* grad_logits,
+                                           size_t grad_stride, size_t rows, int vocab, float inv_temperature) {
+    switch (type) {
+        case ElementType::F32:
+            return backward<float>(stream, logits, stride, tokens, lse, entropy, grad_log_prob, grad_entropy, grad_logits,
+                                   grad_stride, rows, vocab, inv_temperature);
+        case ElementType::F16:
+            return backward<_Float16>(stream, logits, stride, tokens, lse, entropy, grad_log_prob, grad_entropy, grad_logits,
+                                      grad_stride, rows, vocab, inv_temperature);
+        case ElementType::BF16:
+            return backward<__bf16>(stream, logits, stride, tokens, lse, entropy, grad_log_prob, grad_entropy, grad_logits,
+                                    grad_stride, rows, vocab, inv_temperature);
+    }
+    return hipErrorInvalidValue;
+}
+
+}  // namespace mcc

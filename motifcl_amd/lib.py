@@ -38,6 +38,23 @@ SIGNATURES = {
     "mcc_sgd_update_f32": (ctypes.c_int, [_vp, _vp, _sz, _vp, _sz, _sz, _f]),
     "mcc_adam_update_f32": (ctypes.c_int, [_vp, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _sz, _f, _f, _f, _f,
                                            ctypes.c_int, _f]),
+    "mcc_layer_norm": (ctypes.c_int, [_vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _sz, _vp, _sz, _vp, _sz,
+                                      _sz, _sz, ctypes.c_int, _f]),
+    "mcc_layer_norm_backward_workspace_nbytes": (_sz, [_sz, _sz, ctypes.c_int]),
+    "mcc_layer_norm_backward": (
+        ctypes.c_int, [_vp, _vp, _sz, _sz, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _sz, _vp, _sz, _vp,
+                       _sz, _vp, _sz, _sz, _sz, ctypes.c_int]),
+    "mcc_token_log_probs_workspace_nbytes": (_sz, [_sz, _sz, _sz, ctypes.c_int]),
+    "mcc_token_log_probs": (
+        ctypes.c_int, [_vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz,
+                       _sz, _sz, _sz, ctypes.c_int, _f]),
+    "mcc_token_log_probs_backward": (
+        ctypes.c_int, [_vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _sz, _sz, _sz,
+                       ctypes.c_int, _f]),
+    "mcc_distill_top_workspace_nbytes": (_sz, [_sz, _sz, ctypes.c_int]),
+    "mcc_distill_top": (
+        ctypes.c_int, [_vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _sz, _vp, _sz,
+                       _sz, _sz, _sz, ctypes.c_int, _f]),
     "mcc_device_alloc": (ctypes.c_int, [ctypes.POINTER(_vp), _sz]),
     "mcc_device_free": (ctypes.c_int, [_vp]),
     "mcc_device_pool_clear": (ctypes.c_int, []),

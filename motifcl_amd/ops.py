@@ -1,6 +1,7 @@
 """Thin Python front of the C ABI.  torch is used only as the owner of device
 memory and of the current HIP stream; every computation happens in
 libmotifcl_amd.so."""
+import collections
 import ctypes
 
 import torch
@@ -206,6 +207,184 @@ def adam_update(param, grad, m, v, lr, beta1, beta2, eps, step, weight_decay=0.0
     _lib.check(L.mcc_adam_update_f32(_stream(), *_buf(param, torch.float32), *_buf(grad, torch.float32),
                                      *_buf(m, torch.float32), *_buf(v, torch.float32), param.numel(),
                                      lr, beta1, beta2, eps, step, weight_decay))
+
+
+# ---- row-wise operators around the counter layers ------------------------------------------------
+_ELEMENTS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # MCC_ELEMENT_* of include/motifcl_amd.h
+MOST_TOP = 128  # MCC_MOST_TOP
+
+TokenLogProbs = collections.namedtuple("TokenLogProbs", "log_prob entropy lse top_ids top_log_probs")
+
+
+def _rows(t, name):
+    """(pointer, bytes, row stride), rows, row length and element type of a tensor whose last dimension is the
+    row: contiguous, or two-dimensional with contiguous rows."""
+    if not t.is_cuda:
+        raise ValueError("expected a device tensor")
+    element = _ELEMENTS.get(t.dtype)
+    if element is None:
+        raise ValueError("%s: expected float32, float16 or bfloat16, got %s" % (name, t.dtype))
+    if t.dim() == 0:
+        raise ValueError("%s: expected at least one dimension" % name)
+    cols = t.shape[-1]
+    rows = t.numel() // cols if cols else 0
+    stride = cols
+    if not t.is_contiguous():
+        if t.dim() != 2 or (t.stride(1) != 1 and cols != 1):
+            raise ValueError("%s: expected a contiguous tensor or a matrix with contiguous rows" % name)
+        stride = t.stride(0)
+    size = 4 if element == 0 else 2
+    nbytes = ((rows - 1) * stride + cols) * size if rows else 0
+    return (t.data_ptr(), nbytes, stride), rows, cols, element
+
+
+def _same_rows(t, like, name):
+    """(pointer, bytes, row stride) of a tensor with the shape, type and device of `like`."""
+    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+        raise ValueError("%s: expected shape %s, %s on %s" % (name, tuple(like.shape), like.dtype, like.device))
+    return _rows(t, name)[0]
+
+
+def _numbers(t, dtype, shape, like, name):
+    """(pointer, bytes) of a contiguous tensor on the device of `like`; None gives a null pointer."""
+    if t is None:
+        return None, 0
+    if t.shape != shape or t.device != like.device:
+        raise ValueError("%s: expected shape %s on %s, got %s on %s" % (name, tuple(shape), like.device, tuple(t.shape),
+                                                                       t.device))
+    return _buf(t, dtype)
+
+
+def _call(fn, like, *args):
+    """One call on the current stream of the device that `like` is on."""
+    device = like.device
+    stream = torch.cuda.current_stream(device).cuda_stream or None
+    if device.index == torch.cuda.current_device():
+        _lib.check(fn(stream, *args))
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn(stream, *args))
+
+
+def _lent(nbytes, workspace, like):
+    """(pointer, bytes) and owner of a workspace: the caller's, or a new one (None if none is needed)."""
+    if workspace is None:
+        if nbytes == 0:
+            return (None, 0), None
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    elif workspace.device != like.device:
+        raise ValueError("workspace: expected a tensor on %s" % like.device)
+    return _buf(workspace, torch.uint8), workspace
+
+
+def layer_norm(x, gain=None, bias=None, eps=1e-5, out=None):
+    """Layer norm of the rows (last dimension) of x: (y, mean, rstd).  gain and bias are float32 vectors;
+    `out` may be x."""
+    buf, rows, cols, element = _rows(x, "x")
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    _call(_lib.load().mcc_layer_norm, x, *buf, *_numbers(gain, torch.float32, (cols,), x, "gain"),
+          *_numbers(bias, torch.float32, (cols,), x, "bias"), *_same_rows(y, x, "out"),
+          mean.data_ptr(), 4 * rows, rstd.data_ptr(), 4 * rows, rows, cols, element, eps)
+    return y, mean, rstd
+
+
+def layer_norm_backward_workspace_nbytes(rows, cols, dtype):
+    return int(_lib.load().mcc_layer_norm_backward_workspace_nbytes(rows, cols, _ELEMENTS[dtype]))
+
+
+def layer_norm_backward(grad_out, x, mean, rstd, gain=None, bias=True, input_grad=True, out=None, workspace=None):
+    """Gradients of layer_norm: (grad_x, grad_gain, grad_bias).  grad_gain is None without a gain, grad_bias with
+    bias=False, grad_x with input_grad=False; `out` takes grad_x and may be grad_out or x."""
+    L = _lib.load()
+    buf, rows, cols, element = _rows(x, "x")
+    grad_buf = _same_rows(grad_out, x, "grad_out")
+    grad_x = None
+    if input_grad:
+        grad_x = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+    x_out = _same_rows(grad_x, x, "out") if input_grad else (None, 0, 0)
+    grad_gain = torch.empty(cols, dtype=torch.float32, device=x.device) if gain is not None else None
+    grad_bias = torch.empty(cols, dtype=torch.float32, device=x.device) if bias else None
+    need = 0 if grad_gain is None and grad_bias is None else L.mcc_layer_norm_backward_workspace_nbytes(rows, cols, element)
+    lent, workspace = _lent(need, workspace, x)
+    _call(L.mcc_layer_norm_backward, x, *grad_buf, *buf, *_numbers(mean, torch.float32, x.shape[:-1], x, "mean"),
+          *_numbers(rstd, torch.float32, x.shape[:-1], x, "rstd"), *_numbers(gain, torch.float32, (cols,), x, "gain"),
+          *x_out, *_numbers(grad_gain, torch.float32, (cols,), x, "grad_gain"),
+          *_numbers(grad_bias, torch.float32, (cols,), x, "grad_bias"), *lent, rows, cols, element)
+    return grad_x, grad_gain, grad_bias
+
+
+def token_log_probs_workspace_nbytes(rows, vocab, top, dtype):
+    return int(_lib.load().mcc_token_log_probs_workspace_nbytes(rows, vocab, top, _ELEMENTS[dtype]))
+
+
+def token_log_probs(logits, tokens=None, top=0, temperature=1.0, workspace=None):
+    """TokenLogProbs of softmax(logits / temperature) along the last dimension: the log probability of `tokens`
+    (int32, one a row; outside the vocabulary: 0; None without tokens), the entropy, the log of the sum of
+    exponentials, and the `top` likeliest tokens with their log probabilities (None without)."""
+    L = _lib.load()
+    buf, rows, vocab, element = _rows(logits, "logits")
+    shape, device = logits.shape[:-1], logits.device
+    token_buf = _numbers(tokens, torch.int32, shape, logits, "tokens")
+    log_prob = torch.empty(shape, dtype=torch.float32, device=device) if tokens is not None else None
+    entropy = torch.empty(shape, dtype=torch.float32, device=device)
+    lse = torch.empty(shape, dtype=torch.float32, device=device)
+    ids = best = None
+    if 0 < top <= MOST_TOP:
+        ids = torch.empty((*shape, top), dtype=torch.int32, device=device)
+        best = torch.empty((*shape, top), dtype=torch.float32, device=device)
+    lent, workspace = _lent(L.mcc_token_log_probs_workspace_nbytes(rows, vocab, top, element) if top >= 0 else 0,
+                            workspace, logits)
+    n = 4 * rows
+    _call(L.mcc_token_log_probs, logits, *buf, *token_buf,
+          None if log_prob is None else log_prob.data_ptr(), n, entropy.data_ptr(), n, lse.data_ptr(), n,
+          None if ids is None else ids.data_ptr(), n * top, None if best is None else best.data_ptr(), n * top,
+          *lent, rows, vocab, top, element, temperature)
+    return TokenLogProbs(log_prob, entropy, lse, ids, best)
+
+
+def token_log_probs_backward(logits, tokens, lse, entropy, grad_log_prob, grad_entropy=None, temperature=1.0, out=None):
+    """Gradient of the logits from the gradients of token_log_probs' log_prob and entropy (either may be None);
+    lse and entropy are its results.  `out` may be logits."""
+    buf, rows, vocab, element = _rows(logits, "logits")
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if out is None else out
+    shape = logits.shape[:-1]
+    f32 = torch.float32
+    _call(_lib.load().mcc_token_log_probs_backward, logits, *buf, *_numbers(tokens, torch.int32, shape, logits, "tokens"),
+          *_numbers(lse, f32, shape, logits, "lse"), *_numbers(entropy, f32, shape, logits, "entropy"),
+          *_numbers(grad_log_prob, f32, shape, logits, "grad_log_prob"),
+          *_numbers(grad_entropy, f32, shape, logits, "grad_entropy"), *_same_rows(grad, logits, "out"),
+          rows, vocab, element, temperature)
+    return grad
+
+
+def distill_top_workspace_nbytes(rows, vocab, dtype):
+    return int(_lib.load().mcc_distill_top_workspace_nbytes(rows, vocab, _ELEMENTS[dtype]))
+
+
+def distill_top(logits, teacher_ids, teacher_logits, temperature=1.0, weight=None, grad=True, out=None, workspace=None):
+    """Distillation from a teacher's top logits: (loss, grad_logits).  loss is temperature^2 * KL(teacher || student)
+    of each row, grad_logits the gradient of sum(weight * loss) (None with grad=False).  teacher_ids (int32, an id
+    outside the vocabulary is no entry) and teacher_logits (float32) hold the same number of entries a row, at most
+    128; `out` takes grad_logits and may be logits."""
+    L = _lib.load()
+    buf, rows, vocab, element = _rows(logits, "logits")
+    shape, device = logits.shape[:-1], logits.device
+    if teacher_ids.dim() == 0:
+        raise ValueError("teacher_ids: expected [..., entries]")
+    top = teacher_ids.shape[-1]
+    loss = torch.empty(shape, dtype=torch.float32, device=device)
+    grad_logits = None
+    if grad:
+        grad_logits = torch.empty(logits.shape, dtype=logits.dtype, device=device) if out is None else out
+    grad_buf = _same_rows(grad_logits, logits, "out") if grad else (None, 0, 0)
+    lent, workspace = _lent(L.mcc_distill_top_workspace_nbytes(rows, vocab, element), workspace, logits)
+    _call(L.mcc_distill_top, logits, *buf, *_numbers(teacher_ids, torch.int32, (*shape, top), logits, "teacher_ids"),
+          *_numbers(teacher_logits, torch.float32, (*shape, top), logits, "teacher_logits"),
+          *_numbers(weight, torch.float32, shape, logits, "weight"), loss.data_ptr(), 4 * rows, *grad_buf, *lent,
+          rows, vocab, top, element, temperature)
+    return loss, grad_logits
 
 
 CONTRACTION_FP32, CONTRACTION_BF16X6 = 0, 1
