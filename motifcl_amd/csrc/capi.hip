@@ -944,7 +944,7 @@ struct RowsCheck {
         return say(std::string(out_name) + " overlaps " + in_name);
     }
     bool temperature(float t) const {
-        if (!std::isfinite(t) || !(t > 0.0f) || !std::isfinite(1.0f / t)) return say("requires a positive finite temperature");
+        if (!std::isfinite(t) || !(t > 0.0f) || !std::isfinite(2.0f / t)) return say("requires a positive finite temperature");
         return true;
     }
     // workgroups of one launch
@@ -953,7 +953,9 @@ struct RowsCheck {
     }
 };
 
-// Rows are cut into stretches of no less than 4096 elements.
+float log2_scale(float temperature) { return (float)(1.44269504088896340736 / (double)temperature); }
+
+// No kernel cuts rows into stretches shorter than 4096 elements.
 size_t most_stretches(size_t cols) { return (cols + 4095) / 4096; }
 
 }  // namespace
@@ -1012,7 +1014,7 @@ int mcc_layer_norm_backward(void* stream, const void* grad_out, size_t grad_out_
 size_t mcc_token_log_probs_workspace_nbytes(size_t rows, size_t vocab, size_t top, int element) {
     RowsCheck c{"token_log_probs", rows, vocab};
     if (!c.shape(element) || top > MCC_MOST_TOP || top > vocab || !c.groups(most_stretches(vocab))) return 0;
-    return mcc::token_log_probs_workspace_nbytes(c.type, rows, (int)vocab, (int)top);
+    return mcc::token_log_probs_workspace_nbytes(rows, (int)vocab, (int)top);
 }
 
 int mcc_token_log_probs(void* stream, const void* logits, size_t logits_nbytes, size_t logits_stride,
@@ -1030,10 +1032,10 @@ int mcc_token_log_probs(void* stream, const void* logits, size_t logits_nbytes, 
         !c.numbers("entropy", entropy, entropy_nbytes, rows, true) || !c.numbers("lse", lse, lse_nbytes, rows, true) ||
         !c.numbers("top_ids", top_ids, top_ids_nbytes, rows * top, true) ||
         !c.numbers("top_log_probs", top_log_probs, top_log_probs_nbytes, rows * top, true) ||
-        !c.workspace(workspace, workspace_nbytes, mcc::token_log_probs_workspace_nbytes(c.type, rows, (int)vocab, (int)top)))
+        !c.workspace(workspace, workspace_nbytes, mcc::token_log_probs_workspace_nbytes(rows, (int)vocab, (int)top)))
         return MCC_E_INVALID;
-    const mcc::TokenLogProbs a{logits, logits_stride, rows, (int)vocab, (int)top, 1.0f / temperature, tokens,
-                               log_prob, entropy, lse, top_ids, top_log_probs};
+    const mcc::TokenLogProbs a{logits, logits_stride, rows, (int)vocab, (int)top, 1.0f / temperature,
+                               log2_scale(temperature), tokens, log_prob, entropy, lse, top_ids, top_log_probs};
     ScopedKernelTimer timer("token_log_probs", static_cast<hipStream_t>(stream));
     const hipError_t e = mcc::launch_token_log_probs(static_cast<hipStream_t>(stream), c.type, a, workspace);
     if (e != hipSuccess) return hip_fail(e, "token_log_probs launch failed");
@@ -1069,7 +1071,7 @@ int mcc_token_log_probs_backward(void* stream, const void* logits, size_t logits
 size_t mcc_distill_top_workspace_nbytes(size_t rows, size_t vocab, int element) {
     RowsCheck c{"distill_top", rows, vocab};
     if (!c.shape(element) || !c.groups(most_stretches(vocab))) return 0;
-    return mcc::distill_top_workspace_nbytes(c.type, rows, (int)vocab);
+    return mcc::distill_top_workspace_nbytes(rows, (int)vocab);
 }
 
 int mcc_distill_top(void* stream, const void* logits, size_t logits_nbytes, size_t logits_stride,
@@ -1091,10 +1093,10 @@ int mcc_distill_top(void* stream, const void* logits, size_t logits_nbytes, size
         return MCC_E_INVALID;
     if (grad_logits && (!c.tensor("grad_logits", ga) || !c.apart("grad_logits", ga, "logits", la))) return MCC_E_INVALID;
     if (!loss && !grad_logits) return fail(MCC_E_INVALID, "distill_top received no output");
-    if (!c.workspace(workspace, workspace_nbytes, mcc::distill_top_workspace_nbytes(c.type, rows, (int)vocab)))
+    if (!c.workspace(workspace, workspace_nbytes, mcc::distill_top_workspace_nbytes(rows, (int)vocab)))
         return MCC_E_INVALID;
     const mcc::DistillTop a{logits, logits_stride, rows, (int)vocab, (int)top, temperature, 1.0f / temperature,
-                            teacher_ids, teacher_logits, weight, loss, grad_logits, grad_logits_stride};
+                            log2_scale(temperature), teacher_ids, teacher_logits, weight, loss, grad_logits, grad_logits_stride};
     ScopedKernelTimer timer("distill_top", static_cast<hipStream_t>(stream));
     const hipError_t e = mcc::launch_distill_top(static_cast<hipStream_t>(stream), c.type, a, workspace);
     if (e != hipSuccess) return hip_fail(e, "distill_top launch failed");

@@ -2,8 +2,8 @@
 // vocabulary and q = softmax(y / T) over the teacher's entries (id, y) of the row,
 //     loss = T^2 sum q_i (log q_i - log p_id(i)),   d(weight loss)/dz_j = weight T (p_j sum q - sum over id(i) = j of q_i)
 // sum q is 1, or 0 in a row without entries.  Bound by memory: the logits are read once and the gradient
-// is written once.  A workgroup that holds its row in registers does both in one launch; longer rows and
-// rows too few to fill the device are cut into stretches: statistics of the stretches, then the rows'
+// is written once.  A workgroup that holds its row in registers does both in one launch; longer rows
+// are cut into stretches: statistics of the stretches, then the rows'
 // losses, then the gradient from a second read.  The teacher's entries change `top` elements of a row: the
 // gradient is written without them first and those elements are written again by the same workgroup
 // behind a barrier, each by the first of the entries that name it.
@@ -51,7 +51,7 @@ __device__ __forceinline__ void weigh_entries(const DistillTop& a, Entries& e) {
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
         e.log_q[i] = (e.y[i] - largest) * a.inv_temperature;
-        e.q[i] = fast_exp(e.log_q[i]);
+        e.q[i] = exp2_of(e.log_q[i] * kLog2E);
         sum += e.q[i];
     }
     sum = wave_reduce<Sum>(sum);
@@ -92,7 +92,7 @@ struct PatchScratch {
     }
 };
 
-// Gradient of a stretch whose logits are in registers: v = c e^((z - m) / T), and the teacher's entries in
+// Gradient of a stretch whose logits are in registers: v = c 2^((z - m) k), and the teacher's entries in
 // it once more, by the first wave.  A barrier lies between lds.put() and this.
 template <typename T, int THREADS, int ITERS>
 __device__ __forceinline__ void write_gradient(const DistillTop& a, size_t row, int from, int n,
@@ -109,7 +109,7 @@ __device__ __forceinline__ void write_gradient(const DistillTop& a, size_t row, 
         float v[Row::kVec];
 #pragma unroll
         for (int k = 0; k < Row::kVec; ++k)
-            v[k] = zero ? 0.0f : c * fast_exp(((float)r.raw[j][k] - base) * a.inv_temperature);
+            v[k] = zero ? 0.0f : c * exp2_of(((float)r.raw[j][k] - base) * a.log2_scale);
         store_row_vector<T, THREADS, ITERS>(out + from, j, t, n, v);
     }
     __syncthreads();
@@ -124,7 +124,7 @@ __device__ __forceinline__ void write_gradient(const DistillTop& a, size_t row, 
                 q += lds.q[other];
                 first = first && other >= at;
             }
-        if (first) out[id] = (T)(c * fast_exp((lds.z[at] - base) * a.inv_temperature) - scale * q);
+        if (first) out[id] = (T)(c * exp2_of((lds.z[at] - base) * a.log2_scale) - scale * q);
     }
 }
 
@@ -147,7 +147,7 @@ __global__ __launch_bounds__(THREADS) void distill_row_kernel(DistillTop a) {
     }
     r.fill_tail(t, n, (T)-__builtin_inff());
     float thread_max;
-    const SoftmaxStats st = stats_of<Row, kWaves, kIters>(r, a.inv_temperature, slots, wave, lane, thread_max);
+    const SoftmaxStats st = stats_of<Row, kWaves, kIters>(r, a.log2_scale, slots, wave, lane, thread_max);
     if (wave == 0 && a.loss) {
         const float loss = loss_of(a, e, st.m, st.s);
         if (lane == 0) a.loss[row] = loss;
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(64) void distill_loss_kernel(DistillTop a, int segm
     const size_t row = blockIdx.x;
     Entries e = load_entries<T>(a, row, 0, a.vocab, threadIdx.x);
     SoftmaxStats st = stats[row * segments];
-    for (int i = 1; i < segments; ++i) st = join_stats(st, stats[row * segments + i], a.inv_temperature);
+    for (int i = 1; i < segments; ++i) st = join_stats(st, stats[row * segments + i], a.log2_scale);
     weigh_entries(a, e);
     const float loss = loss_of(a, e, st.m, st.s);
     if (threadIdx.x == 0) {
@@ -194,38 +194,35 @@ __global__ __launch_bounds__(THREADS) void distill_gradient_kernel(DistillTop a,
 
 template <typename T>
 hipError_t distill(hipStream_t stream, ElementType type, const DistillTop& a, void* workspace) {
-    const RowCut c = cut_rows(a.rows, a.vocab);
-    SoftmaxStats* stats = static_cast<SoftmaxStats*>(workspace);
-#define MCC_DISTILL(THREADS, PER_THREAD)                                                                                 \
-    if (c.threads == THREADS && c.per_thread == PER_THREAD) {                                                            \
-        if (c.segments == 1)                                                                                             \
-            hipLaunchKernelGGL((distill_row_kernel<T, THREADS, PER_THREAD>), dim3((unsigned)a.rows), dim3(THREADS), 0,    \
-                               stream, a);                                                                               \
-        else                                                                                                             \
-            hipLaunchKernelGGL((distill_gradient_kernel<T, THREADS, PER_THREAD>), dim3((unsigned)(a.rows * c.segments)), \
-                               dim3(THREADS), 0, stream, a, c.segments, c.length, stats);                                \
-    }
+    const RowCut c = cut_rows(a.vocab);
     if (c.segments > 1) {
-        hipError_t e = launch_softmax_stats(stream, type, a.logits, a.stride, a.rows, a.vocab, a.inv_temperature, c, stats);
+        SoftmaxStats* stats = static_cast<SoftmaxStats*>(workspace);
+        hipError_t e = launch_softmax_stats(stream, type, a.logits, a.stride, a.rows, a.vocab, a.log2_scale, c, stats);
         if (e != hipSuccess) return e;
         hipLaunchKernelGGL(distill_loss_kernel<T>, dim3((unsigned)a.rows), dim3(64), 0, stream, a, c.segments, stats);
         e = hipGetLastError();
         if (e != hipSuccess || !a.grad) return e;
+        hipLaunchKernelGGL((distill_gradient_kernel<T, 1024, 32>), dim3((unsigned)(a.rows * c.segments)), dim3(1024), 0,
+                           stream, a, c.segments, c.length, stats);
+        return hipGetLastError();
     }
-    MCC_DISTILL(64, 8)
-    MCC_DISTILL(64, 32)
-    MCC_DISTILL(256, 16)
-    MCC_DISTILL(256, 32)
-    MCC_DISTILL(512, 32)
-    MCC_DISTILL(1024, 32)
+#define MCC_DISTILL(THREADS, PER_THREAD)                                                                              \
+    if (c.threads == THREADS && c.per_thread == PER_THREAD)                                                           \
+    hipLaunchKernelGGL((distill_row_kernel<T, THREADS, PER_THREAD>), dim3((unsigned)a.rows), dim3(THREADS), 0, stream, a)
+    MCC_DISTILL(64, 8);
+    MCC_DISTILL(64, 32);
+    MCC_DISTILL(256, 16);
+    MCC_DISTILL(256, 32);
+    MCC_DISTILL(512, 32);
+    MCC_DISTILL(1024, 32);
 #undef MCC_DISTILL
     return hipGetLastError();
 }
 
 }  // namespace
 
-size_t distill_top_workspace_nbytes(ElementType, size_t rows, int vocab) {
-    const RowCut c = cut_rows(rows, vocab);
+size_t distill_top_workspace_nbytes(size_t rows, int vocab) {
+    const RowCut c = cut_rows(vocab);
     return c.segments == 1 ? 0 : rows * c.segments * sizeof(SoftmaxStats);
 }
 

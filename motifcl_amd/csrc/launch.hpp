@@ -173,13 +173,13 @@ struct TokenLogProbs {
     const void* logits;
     size_t stride, rows;
     int vocab, top;
-    float inv_temperature;
+    float inv_temperature, log2_scale;  // 1 / temperature and log2(e) / temperature
     const int32_t* tokens;
     float *log_prob, *entropy, *lse;
     int32_t* top_ids;
     float* top_log_probs;
 };
-size_t token_log_probs_workspace_nbytes(ElementType type, size_t rows, int vocab, int top);
+size_t token_log_probs_workspace_nbytes(size_t rows, int vocab, int top);
 hipError_t launch_token_log_probs(hipStream_t stream, ElementType type, const TokenLogProbs& a, void* workspace);
 hipError_t launch_token_log_probs_backward(hipStream_t stream, ElementType type, const void* logits, size_t stride,
                                            const int32_t* tokens, const float* lse, const float* entropy,
@@ -192,7 +192,7 @@ struct DistillTop {
     const void* logits;
     size_t stride, rows;
     int vocab, top;
-    float temperature, inv_temperature;
+    float temperature, inv_temperature, log2_scale;
     const int32_t* ids;      // [rows, top], outside [0, vocab): no entry
     const float* teacher;    // [rows, top]
     const float* weight;     // [rows]
@@ -200,7 +200,7 @@ struct DistillTop {
     void* grad;
     size_t grad_stride;
 };
-size_t distill_top_workspace_nbytes(ElementType type, size_t rows, int vocab);
+size_t distill_top_workspace_nbytes(size_t rows, int vocab);
 hipError_t launch_distill_top(hipStream_t stream, ElementType type, const DistillTop& a, void* workspace);
 
 }  // namespace mcc

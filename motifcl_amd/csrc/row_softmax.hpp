@@ -1,9 +1,8 @@
 // The softmax statistics of a stretch of a row in registers, and how a row is cut into stretches.
-// With d = (z - max) / temperature over the stretch:
-//     m = max z,  s = sum e^d,  u = sum e^d d
-// from which log sum e^(z / temperature) = m / temperature + log s and the entropy is log s - u / s.
-// Stretches are joined by m = max m_i, r_i = e^((m_i - m) / temperature), s = sum r_i s_i,
-// u = sum r_i (u_i + s_i (m_i - m) / temperature).  A stretch of -inf alone has m = -inf, s = u = 0; a NaN or
+// With d = (z - max) k and k = log2(e) / temperature over the stretch:
+//     m = max z,  s = sum 2^d,  u = sum 2^d d
+// from which log sum e^(z / temperature) = m / temperature + log s and the entropy is log s - log(2) u / s.
+// Stretches are joined by m = max m_i, r_i = 2^((m_i - m) k), s = sum r_i s_i, u = sum r_i (u_i + s_i (m_i - m) k).  A stretch of -inf alone has m = -inf, s = u = 0; a NaN or
 // +inf makes s (and with it everything taken from the row) NaN.
 #pragma once
 
@@ -25,17 +24,17 @@ struct SoftmaxStats {
 __device__ __forceinline__ float shift_of(float m) { return m == -__builtin_inff() ? 0.0f : m; }
 
 // a joined to b; the order of the operands is the order of the stretches
-__device__ __forceinline__ SoftmaxStats join_stats(SoftmaxStats a, SoftmaxStats b, float inv_temperature) {
+__device__ __forceinline__ SoftmaxStats join_stats(SoftmaxStats a, SoftmaxStats b, float k) {
     const float m = fmaxf(a.m, b.m), base = shift_of(m);
-    const float da = (a.m - base) * inv_temperature, db = (b.m - base) * inv_temperature;
-    const float ra = fast_exp(da), rb = fast_exp(db);
+    const float da = (a.m - base) * k, db = (b.m - base) * k;
+    const float ra = exp2_of(da), rb = exp2_of(db);
     // an empty stretch has d = -inf: its sums are zero and stay so
     return {m, ra * a.s + rb * b.s, ra * (a.u + a.s * fmaxf(da, -1e4f)) + rb * (b.u + b.s * fmaxf(db, -1e4f))};
 }
 
-// slots: 3 * WAVES floats of LDS that no wave still reads
+// scale is k above; slots: 3 * WAVES floats of LDS that no wave still reads
 template <typename ROW, int WAVES, int ITERS>
-__device__ __forceinline__ SoftmaxStats stats_of(const ROW& r, float inv_temperature, float* slots, int wave, int lane,
+__device__ __forceinline__ SoftmaxStats stats_of(const ROW& r, float scale, float* slots, int wave, int lane,
                                                  float& thread_max) {
     SoftmaxStats st;
     float largest[1] = {-__builtin_inff()};
@@ -52,7 +51,7 @@ __device__ __forceinline__ SoftmaxStats stats_of(const ROW& r, float inv_tempera
     for (int j = 0; j < ITERS; ++j)
 #pragma unroll
         for (int k = 0; k < ROW::kVec; ++k) {
-            const float d = ((float)r.raw[j][k] - base) * inv_temperature, e = fast_exp(d);
+            const float d = ((float)r.raw[j][k] - base) * scale, e = exp2_of(d);
             sums[0] += e;
             sums[1] = fmaf(e, fmaxf(d, -1e4f), sums[1]);  // e is 0 long before the bound: 0 * -inf does not arise
         }
@@ -67,30 +66,28 @@ __device__ __forceinline__ SoftmaxStats stats_of(const ROW& r, float inv_tempera
 struct RowCut {
     int threads, per_thread, segments, length;
 };
-// Workgroups that fill the device: two a CU.
-constexpr size_t kFillGroups = 512;
-inline RowCut cut_rows(size_t rows, int vocab) {
-    // as long stretches as a workgroup's registers hold, shorter ones while the rows are too few to give every CU
-    // work, but not under 4096 numbers: joining more stretches then costs what their loads save
-    int most = 32768;
-    while (most > 4096 && rows * (size_t)((vocab + (size_t)most - 1) / most) < kFillGroups) most /= 2;
+constexpr int kMostHeld = 32768;  // numbers in the registers of a workgroup of 1024 threads
+// Rows are cut only where a workgroup cannot hold one.  Cutting few rows further, so that more CUs read
+// them, does not pay for the launch that joins the stretches: one row of 32768 f32 takes 30.7 us from call to
+// end whole and 34.6 us in eight stretches, 200 rows 35 and 39 us, one row of 128011 37 us in four stretches
+// and 45 us in 32.
+inline RowCut cut_rows(int vocab) {
     RowCut c;
-    c.segments = (int)(((size_t)vocab + most - 1) / most);
+    c.segments = (int)(((size_t)vocab + kMostHeld - 1) / kMostHeld);
     const size_t even = ((size_t)vocab + c.segments - 1) / c.segments;
     c.length = (int)((even + 7) / 8 * 8);  // stretches begin where 16-byte accesses of an aligned row do
-    c.segments = (int)(((size_t)vocab + c.length - 1) / c.length);
-    const int n = c.length < vocab ? c.length : vocab;
-    if (n <= 512) c.threads = 64, c.per_thread = 8;
-    else if (n <= 2048) c.threads = 64, c.per_thread = 32;
-    else if (n <= 4096) c.threads = 256, c.per_thread = 16;
-    else if (n <= 8192) c.threads = 256, c.per_thread = 32;
-    else if (n <= 16384) c.threads = 512, c.per_thread = 32;
+    if (c.segments > 1) c.threads = 1024, c.per_thread = 32;  // longer than half of what it holds
+    else if (vocab <= 512) c.threads = 64, c.per_thread = 8;
+    else if (vocab <= 2048) c.threads = 64, c.per_thread = 32;
+    else if (vocab <= 4096) c.threads = 256, c.per_thread = 16;
+    else if (vocab <= 8192) c.threads = 256, c.per_thread = 32;
+    else if (vocab <= 16384) c.threads = 512, c.per_thread = 32;
     else c.threads = 1024, c.per_thread = 32;
     return c;
 }
 
-// Statistics of every stretch of every row: stats[row * segments + segment].
+// Statistics of every stretch of rows that are cut: stats[row * segments + segment].
 hipError_t launch_softmax_stats(hipStream_t stream, ElementType type, const void* logits, size_t stride, size_t rows,
-                                int vocab, float inv_temperature, const RowCut& cut, SoftmaxStats* stats);
+                                int vocab, float log2_scale, const RowCut& cut, SoftmaxStats* stats);
 
 }  // namespace mcc

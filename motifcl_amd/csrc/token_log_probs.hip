@@ -1,9 +1,9 @@
 // Log probabilities of given tokens under softmax(logits / temperature), the entropy of that
 // distribution, its `top` likeliest tokens, and the gradient of the logits.
-//     log p_j = (z_j - m) / T - log s,  H = log s - u / s               (row_softmax.hpp)
+//     log p_j = (z_j - m) / T - log s,  H = log s - log(2) u / s        (row_softmax.hpp)
 //     dz_j = (g (delta_j,token - p_j) - h p_j (log p_j + H)) / T        for upstream gradients g of log p and h of H
 // Bound by memory: the logits are read once, into registers, by one workgroup a row or, where rows are
-// long or few, by one a stretch of a row; a second launch then joins the stretches.  The top entries are
+// longer than it can hold, a stretch of a row; a second launch then joins the stretches.  The top entries are
 // found in the registers: numbers below a bound that at least `top` numbers reach are passed over, and
 // the few that are left are ranked.  Order: larger logit first, among equals the lower token, -0 = +0,
 // NaN behind -inf; so equal calls give equal bytes whatever order the candidates were found in.
@@ -34,121 +34,147 @@ __device__ __forceinline__ float of_key(uint32_t k) {
 // A candidate: larger is likelier, and among equal logits the lower token is larger.
 __device__ __forceinline__ uint64_t candidate(float z, uint32_t id) { return (uint64_t)key_of(z) << 32 | (uint32_t)~id; }
 
-constexpr int kCandidates = 512;
+// The same number, which the compiler takes for a new one: indexes computed from it are computed where they are
+// needed instead of being held in registers since the loads.
+__device__ __forceinline__ int again(int t) {
+    asm volatile("" : "+v"(t));
+    return t;
+}
+
 template <int WAVES>
 struct TopScratch {
+    static constexpr int kCandidates = WAVES == 1 ? 256 : 512;
     uint64_t list[kCandidates];
-    uint32_t bound[WAVES];
+    int rank[kCandidates];
+    uint32_t bound;
     int count;
-    int totals[2][WAVES];
+    float totals[2][WAVES], least[WAVES];
 };
 
 // Sum over the workgroup of a count per wave; `turn` alternates between calls.
 template <int WAVES>
-__device__ __forceinline__ int total_of(int wave_count, int (&totals)[2][WAVES], int turn, int wave, int lane) {
+__device__ __forceinline__ int total_of(int wave_count, float (&totals)[2][WAVES], int turn, int wave, int lane) {
     if (WAVES == 1) return wave_count;
-    if (lane == 0) totals[turn][wave] = wave_count;
+    if (lane == 0) totals[turn][wave] = (float)wave_count;
     __syncthreads();
-    int a = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) a += totals[turn][w];
-    return a;
+    return (int)wave_reduce<Sum>(lane < WAVES ? totals[turn][lane] : 0.0f);  // whole numbers below 2^24
 }
 
-// A number that at least `top` of the workgroup's numbers reach, as a float: every wave gives the
-// ceil(top / WAVES)-th largest of its lanes' maxima (rounded down to a multiple of 64 units of the key,
-// which makes room for the lane), and the smallest of those is reached by as many lanes of every wave.
+// A number that at least `top` of the workgroup's numbers reach: every wave gives the ceil(top / WAVES)-th
+// largest of its lanes' maxima, rounded down to the leading 20 bits of its key (one compare and one
+// population count a bit, the rest scalar), and the smallest of those is reached by as many lanes of
+// every wave.  lds.bound is all ones before.
 template <int WAVES>
-__device__ __forceinline__ float lower_bound_of(float thread_max, int top, TopScratch<WAVES>& lds, int wave, int lane) {
+__device__ __forceinline__ float lower_bound_of(float thread_max, int top, TopScratch<WAVES>& lds, int lane) {
     const int nth = (top + WAVES - 1) / WAVES;
-    const uint32_t mine = (key_of(thread_max) & ~63u) | (uint32_t)(63 - lane);
-    int above = 0;
-#pragma unroll
-    for (int i = 0; i < 64; ++i) above += (uint32_t)__builtin_amdgcn_readlane((int)mine, i) > mine ? 1 : 0;
+    const uint32_t mine = key_of(thread_max);
     uint32_t bound = 0;
-    if (nth <= 64) {
-        const uint64_t there = __builtin_amdgcn_ballot_w64(above == nth - 1);
-        bound = (uint32_t)__builtin_amdgcn_readlane((int)mine, __builtin_ctzll(there)) & ~63u;
+#pragma unroll
+    for (int bit = 31; bit >= 12; --bit) {
+        const uint32_t next = bound | 1u << bit;
+        if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(mine >= next)) >= nth) bound = next;
     }
     if (WAVES > 1) {
-        if (lane == 0) lds.bound[wave] = bound;
+        if (lane == 0) atomicMin(&lds.bound, bound);
         __syncthreads();
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) bound = lds.bound[w] < bound ? lds.bound[w] : bound;
+        bound = lds.bound;
     }
     return bound <= kKeyLowest ? -__builtin_inff() : of_key(bound);
 }
 
 // The `top` candidates of a stretch into lds.list[0 .. top) when too many numbers (ties, as of masked
-// logits) reach the bound, or too few (NaN): the top-th largest key by bisection over its bits, the
-// numbers above it, and the first of those equal to it.
+// logits) reach the bound, or too few (NaN): the top-th largest number, the numbers above it, and the
+// first of those equal to it.  The smallest number that reaches the bound is tried first: in rows with
+// fewer allowed tokens than `top` it is what the others were masked with.  Else the number is found by
+// bisection over the bits of its key.
 template <typename ROW, int WAVES, int ITERS>
-__device__ __forceinline__ void select_by_bisection(const ROW& r, int n, uint32_t first_id, int top, TopScratch<WAVES>& lds,
-                                                 int t, int wave, int lane) {
+__device__ __forceinline__ void select_among_ties(const ROW& r, int n, uint32_t first_id, int top, float bound,
+                                                  TopScratch<WAVES>& lds, int t, int wave, int lane) {
     int turn = 0;
     auto count = [&](auto test) {
         int c = 0;
 #pragma unroll
-        for (int j = 0; j < ITERS; ++j)
+        for (int j = 0; j < ITERS; ++j) {
+            const int u = again(t);
 #pragma unroll
-            for (int k = 0; k < ROW::kVec; ++k) c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(test(j, k)));
+            for (int k = 0; k < ROW::kVec; ++k)
+                c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(test((float)r.raw[j][k], j, k, u)));
+        }
         turn ^= 1;
         return total_of<WAVES>(c, lds.totals, turn, wave, lane);
     };
-    auto value = [&](int j, int k) { return (float)r.raw[j][k]; };
-    const int numbers = count([&](int j, int k) { return value(j, k) >= -__builtin_inff() && ROW::holds(j, k, t, n); });
-    uint32_t key = 0;
-    if (numbers >= top) {
-#pragma unroll 1
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t next = key | 1u << bit;
-            if (next > kKeyHighest) continue;
-            if (next > kKeyLowest) {  // at least `top` numbers reach -inf; above it the filled ones do not count
-                const float f = of_key(next);
-                if (count([&](int j, int k) { return value(j, k) >= f; }) < top) continue;
+    auto number = [&](float z, int j, int k, int u) { return z >= -__builtin_inff() && ROW::holds(j, k, u, n); };
+    float f = 0.0f;
+    const bool numbers = count(number) >= top;  // if not, all numbers are above and NaN are the ties
+    if (numbers) {
+        float least[1] = {__builtin_inff()};
+#pragma unroll
+        for (int j = 0; j < ITERS; ++j)
+#pragma unroll
+            for (int k = 0; k < ROW::kVec; ++k) {
+                const float z = (float)r.raw[j][k];
+                least[0] = z >= bound && z < least[0] ? z : least[0];
             }
-            key = next;
+        least[0] = -wave_reduce<Max>(-least[0]);
+        if (WAVES > 1) {
+            if (lane == 0) lds.least[wave] = least[0];
+            __syncthreads();
+            least[0] = -wave_reduce<Max>(lane < WAVES ? -lds.least[lane] : -__builtin_inff());
+        }
+        f = least[0];
+        if (count([&](float z, int, int, int) { return z > f; }) >= top) {
+            uint32_t key = 0;
+#pragma unroll 1
+            for (int bit = 31; bit >= 0; --bit) {
+                const uint32_t next = key | 1u << bit;
+                if (next > kKeyHighest) continue;
+                if (next > kKeyLowest) {  // at least `top` numbers reach -inf; above it the filled ones do not count
+                    const float g = of_key(next);
+                    if (count([&](float z, int, int, int) { return z >= g; }) < top) continue;
+                }
+                key = next;
+            }
+            f = of_key(key);
         }
     }
-    const float f = key ? of_key(key) : 0.0f;
-    // key 0: all numbers are above, and NaN are the ties
-    auto above = [&](int j, int k) { return key ? value(j, k) > f : value(j, k) >= -__builtin_inff() && ROW::holds(j, k, t, n); };
-    auto equal = [&](int j, int k) { return (key ? value(j, k) == f : !(value(j, k) == value(j, k))) && ROW::holds(j, k, t, n); };
+    auto above = [&](float z, int j, int k, int u) { return numbers ? z > f : number(z, j, k, u); };
+    auto equal = [&](float z, int j, int k, int u) { return (numbers ? z == f : !(z == z)) && ROW::holds(j, k, u, n); };
     const int n_above = count(above);
     __syncthreads();
     if (t == 0) lds.count = 0;
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < ITERS; ++j)
-#pragma unroll
-        for (int k = 0; k < ROW::kVec; ++k)
-            if (above(j, k)) {
-                const int at = atomicAdd(&lds.count, 1);
-                if (at < kCandidates) lds.list[at] = candidate(value(j, k), first_id + ROW::index(j, k, t, n));
-            }
     // ties in the order of their tokens: vector by vector, in it thread by thread
     int before = n_above;
 #pragma unroll
     for (int j = 0; j < ITERS; ++j) {
+        const int u = again(t);
         int of_wave = 0, lower = 0;
         const uint64_t below = ((uint64_t)1 << lane) - 1;
 #pragma unroll
         for (int k = 0; k < ROW::kVec; ++k) {
-            const uint64_t b = __builtin_amdgcn_ballot_w64(equal(j, k));
+            const float z = (float)r.raw[j][k];
+            const uint64_t b = __builtin_amdgcn_ballot_w64(equal(z, j, k, u));
             of_wave += __builtin_popcountll(b);
             lower += __builtin_popcountll(b & below);
+            if (above(z, j, k, u)) {
+                const int at = atomicAdd(&lds.count, 1);
+                if (at < lds.kCandidates) lds.list[at] = candidate(z, first_id + ROW::index(j, k, u, n));
+            }
         }
         turn ^= 1;
         const int all = total_of<WAVES>(of_wave, lds.totals, turn, wave, lane);
         int at = before + lower;
-        for (int w = 0; w < wave; ++w) at += lds.totals[turn][w];
+        for (int w = 0; w < wave; ++w) at += (int)lds.totals[turn][w];
 #pragma unroll
-        for (int k = 0; k < ROW::kVec; ++k)
-            if (equal(j, k)) {
-                if (at < top) lds.list[at] = candidate(value(j, k), first_id + ROW::index(j, k, t, n));
+        for (int k = 0; k < ROW::kVec; ++k) {
+            const float z = (float)r.raw[j][k];
+            if (equal(z, j, k, u)) {
+                if (at < top) lds.list[at] = candidate(z, first_id + ROW::index(j, k, u, n));
                 ++at;
             }
+        }
         before += all;
+        if (before >= top && n_above == 0) break;  // nothing above to look for in the other vectors
     }
     __syncthreads();
 }
@@ -158,26 +184,45 @@ __device__ __forceinline__ void select_by_bisection(const ROW& r, int n, uint32_
 template <typename ROW, int WAVES, int ITERS>
 __device__ __forceinline__ int find_candidates(const ROW& r, int n, uint32_t first_id, int top, float thread_max,
                                                TopScratch<WAVES>& lds, int t, int wave, int lane) {
-    if (t == 0) lds.count = 0;
-    const float bound = lower_bound_of<WAVES>(thread_max, top, lds, wave, lane);
-    if (WAVES == 1) __syncthreads();
+    const float bound = lower_bound_of<WAVES>(thread_max, top, lds, lane);
     if (thread_max >= bound) {
 #pragma unroll
-        for (int j = 0; j < ITERS; ++j)
+        for (int j = 0; j < ITERS; ++j) {
+            const int u = again(t);
 #pragma unroll
             for (int k = 0; k < ROW::kVec; ++k) {
                 const float z = (float)r.raw[j][k];
-                if (z >= bound && ROW::holds(j, k, t, n)) {
+                if (z >= bound && ROW::holds(j, k, u, n)) {
                     const int at = atomicAdd(&lds.count, 1);
-                    if (at < kCandidates) lds.list[at] = candidate(z, first_id + ROW::index(j, k, t, n));
+                    if (at < lds.kCandidates) lds.list[at] = candidate(z, first_id + ROW::index(j, k, u, n));
                 }
             }
+        }
     }
     __syncthreads();
     const int found = lds.count;
-    if (found >= top && found <= kCandidates) return found;
-    select_by_bisection<ROW, WAVES, ITERS>(r, n, first_id, top, lds, t, wave, lane);
+    if (found >= top && found <= lds.kCandidates) return found;
+    select_among_ties<ROW, WAVES, ITERS>(r, n, first_id, top, bound, lds, t, wave, lane);
     return top;
+}
+
+// rank[i] = how many of the n candidates are likelier than list[i].  All the workgroup's threads count: a
+// candidate is compared with a part of the list by each of `parts` threads.
+template <int THREADS>
+__device__ __forceinline__ void rank_candidates(const uint64_t* list, int n, int* rank, int t) {
+    for (int i = t; i < n; i += THREADS) rank[i] = 0;
+    __syncthreads();
+    int parts = 1;
+    while (parts < 16 && 2 * parts * n <= THREADS) parts *= 2;
+    const int width = (n + parts - 1) / parts;
+    for (int at = t; at < n * parts; at += THREADS) {
+        const int i = at % n, from = at / n * width, to = from + width < n ? from + width : n;
+        const uint64_t mine = list[i];
+        int above = 0;
+        for (int k = from; k < to; ++k) above += list[k] > mine ? 1 : 0;
+        if (above) atomicAdd(&rank[i], above);
+    }
+    __syncthreads();
 }
 
 // What is left of a row's statistics once they are joined.
@@ -197,7 +242,7 @@ __device__ __forceinline__ RowResult finish_row(const TokenLogProbs& a, size_t r
     r.inv_temperature = a.inv_temperature;
     if (writes) {
         if (a.lse) a.lse[row] = r.empty ? -__builtin_inff() : st.m * a.inv_temperature + r.log_s;
-        if (a.entropy) a.entropy[row] = r.empty ? 0.0f : r.log_s - st.u / st.s;
+        if (a.entropy) a.entropy[row] = r.empty ? 0.0f : r.log_s - kLn2 * (st.u / st.s);
         if (a.log_prob) a.log_prob[row] = has_token ? r.log_prob(token_logit) : 0.0f;
     }
     return r;
@@ -215,13 +260,14 @@ __device__ __forceinline__ bool token_of(const TokenLogProbs& a, size_t row, flo
 // One stretch a workgroup.  ONE: the row is one stretch, and the results are written; else `stats` and
 // `best` [rows * segments][top] are.
 template <typename T, int THREADS, int PER_THREAD, bool TOP, bool ONE>
-__global__ __launch_bounds__(THREADS) void token_log_probs_kernel(TokenLogProbs a, int segments, int length,
+__global__ __launch_bounds__(THREADS, 8) void token_log_probs_kernel(TokenLogProbs a, int segments, int length,
                                                                   SoftmaxStats* stats, uint64_t* best) {
     constexpr int kIters = PER_THREAD / Elements<T>::kVec, kWaves = THREADS / 64;
     typedef RowVectors<T, THREADS, kIters> Row;
     __shared__ float slots[3 * kWaves];
     __shared__ TopScratch<TOP ? kWaves : 1> lds;
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
+    if (TOP && t == 0) lds.count = 0, lds.bound = ~0u;
     const size_t row = ONE ? blockIdx.x : blockIdx.x / (unsigned)segments;
     const int segment = ONE ? 0 : (int)(blockIdx.x % (unsigned)segments);
     const int from = segment * length, n = a.vocab - from < length ? a.vocab - from : length;
@@ -231,7 +277,7 @@ __global__ __launch_bounds__(THREADS) void token_log_probs_kernel(TokenLogProbs 
     const bool has_token = ONE && t == 0 && token_of<T>(a, row, token_logit);
     r.fill_tail(t, n, (T)-__builtin_inff());
     float thread_max;
-    const SoftmaxStats st = stats_of<Row, kWaves, kIters>(r, a.inv_temperature, slots, wave, lane, thread_max);
+    const SoftmaxStats st = stats_of<Row, kWaves, kIters>(r, a.log2_scale, slots, wave, lane, thread_max);
     RowResult result{};
     if (ONE)
         result = finish_row(a, row, st, token_logit, has_token, t == 0);
@@ -240,10 +286,10 @@ __global__ __launch_bounds__(THREADS) void token_log_probs_kernel(TokenLogProbs 
     if constexpr (TOP) {
         const int top = a.top < n ? a.top : n;
         const int found = find_candidates<Row, kWaves, kIters>(r, n, (uint32_t)from, top, thread_max, lds, t, wave, lane);
+        rank_candidates<THREADS>(lds.list, found, lds.rank, t);
         for (int i = t; i < found; i += THREADS) {
             const uint64_t mine = lds.list[i];
-            int rank = 0;
-            for (int k = 0; k < found; ++k) rank += lds.list[k] > mine ? 1 : 0;
+            const int rank = lds.rank[i];
             if (rank >= top) continue;
             if (ONE) {
                 if (a.top_ids) a.top_ids[row * a.top + rank] = (int32_t)~(uint32_t)mine;
@@ -267,14 +313,15 @@ __global__ __launch_bounds__(kJoinThreads) void token_log_probs_join_kernel(Toke
                                                                            const uint64_t* best) {
     constexpr int kWaves = kJoinThreads / 64;
     __shared__ uint64_t list[kJoinCandidates];
-    __shared__ int count, totals[2][kWaves];
+    __shared__ int ranks[kJoinCandidates], count;
+    __shared__ float totals[2][kWaves];
     __shared__ uint64_t bounds[kWaves];
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     const size_t row = blockIdx.x;
     float token_logit = 0.0f;
     const bool has_token = t == 0 && token_of<T>(a, row, token_logit);
     SoftmaxStats st = stats[row * segments];
-    for (int i = 1; i < segments; ++i) st = join_stats(st, stats[row * segments + i], a.inv_temperature);
+    for (int i = 1; i < segments; ++i) st = join_stats(st, stats[row * segments + i], a.log2_scale);
     const RowResult result = finish_row(a, row, st, token_logit, has_token, t == 0);
     if (a.top == 0 || (!a.top_ids && !a.top_log_probs)) return;
     const uint64_t* entries = best + row * segments * a.top;
@@ -321,10 +368,10 @@ __global__ __launch_bounds__(kJoinThreads) void token_log_probs_join_kernel(Toke
         gather(kth);
         found = count;
     }
+    rank_candidates<kJoinThreads>(list, found, ranks, t);
     for (int i = t; i < found; i += kJoinThreads) {
         const uint64_t mine = list[i];
-        int rank = 0;
-        for (int k = 0; k < found; ++k) rank += list[k] > mine ? 1 : 0;
+        const int rank = ranks[i];
         if (rank >= a.top) continue;
         if (a.top_ids) a.top_ids[row * a.top + rank] = (int32_t)~(uint32_t)mine;
         if (a.top_log_probs) a.top_log_probs[row * a.top + rank] = result.log_prob(of_key((uint32_t)(mine >> 32)));
@@ -354,16 +401,25 @@ __global__ __launch_bounds__(kGradThreads) void token_log_probs_backward_kernel(
     const float h = ENTROPY ? grad_entropy[row] : 0.0f;
     // nothing upstream, or a row of -inf alone: zeros, whatever the logits hold
     const bool zero = (g == 0.0f && h == 0.0f) || l == -__builtin_inff();
+    const float gt = g * inv_temperature, ht = h * inv_temperature;
+    const bool here = token >= from && token - from < n;  // the same for the whole workgroup
 #pragma unroll
     for (int j = 0; j < kIters; ++j) {
         float v[Row::kVec];
 #pragma unroll
         for (int k = 0; k < Row::kVec; ++k) {
-            const float log_p = (float)r.raw[j][k] * inv_temperature - l, p = fast_exp(log_p);
-            float q = -g * p;
-            if (ENTROPY) q -= h * (p * (fmaxf(log_p, -1e4f) + big_h));  // p is 0 long before the bound
-            if (from + Row::index(j, k, t, n) == token) q += g;
-            v[k] = zero ? 0.0f : q * inv_temperature;
+            const float log_p = fmaf((float)r.raw[j][k], inv_temperature, -l), p = exp2_of(log_p * kLog2E);
+            v[k] = -gt * p;
+            if (ENTROPY) v[k] -= ht * (p * (fmaxf(log_p, -1e4f) + big_h));  // p is 0 long before the bound
+        }
+        if (here) {
+#pragma unroll
+            for (int k = 0; k < Row::kVec; ++k)
+                if (from + Row::index(j, k, t, n) == token) v[k] += gt;
+        }
+        if (zero) {
+#pragma unroll
+            for (int k = 0; k < Row::kVec; ++k) v[k] = 0.0f;
         }
         store_row_vector<T, kGradThreads, kIters>(grad_logits + row * grad_stride + from, j, t, n, v);
     }
@@ -372,34 +428,38 @@ __global__ __launch_bounds__(kGradThreads) void token_log_probs_backward_kernel(
 // Workspace of a row cut into stretches: their statistics, then their entries.
 size_t stats_nbytes(size_t rows, const RowCut& c) { return (rows * c.segments * sizeof(SoftmaxStats) + 15) / 16 * 16; }
 
-template <typename T, bool TOP, bool ONE>
+template <typename T, bool TOP>
+hipError_t launch_rows(hipStream_t stream, const TokenLogProbs& a, const RowCut& c) {
+#define MCC_ROWS(THREADS, PER_THREAD)                                                                           \
+    if (c.threads == THREADS && c.per_thread == PER_THREAD)                                                     \
+    hipLaunchKernelGGL((token_log_probs_kernel<T, THREADS, PER_THREAD, TOP, true>), dim3((unsigned)a.rows),     \
+                       dim3(THREADS), 0, stream, a, 1, c.length, (SoftmaxStats*)nullptr, (uint64_t*)nullptr)
+    MCC_ROWS(64, 8);
+    MCC_ROWS(64, 32);
+    MCC_ROWS(256, 16);
+    MCC_ROWS(256, 32);
+    MCC_ROWS(512, 32);
+    MCC_ROWS(1024, 32);
+#undef MCC_ROWS
+    return hipGetLastError();
+}
+
+template <typename T, bool TOP>
 hipError_t launch_stretches(hipStream_t stream, const TokenLogProbs& a, const RowCut& c, SoftmaxStats* stats, uint64_t* best) {
-    const dim3 grid((unsigned)(a.rows * c.segments));
-#define MCC_STRETCH(THREADS, PER_THREAD)                                                                             \
-    if (c.threads == THREADS && c.per_thread == PER_THREAD)                                                          \
-    hipLaunchKernelGGL((token_log_probs_kernel<T, THREADS, PER_THREAD, TOP, ONE>), grid, dim3(THREADS), 0, stream, a, \
-                       c.segments, c.length, stats, best)
-    MCC_STRETCH(64, 8);
-    MCC_STRETCH(64, 32);
-    MCC_STRETCH(256, 16);
-    MCC_STRETCH(256, 32);
-    MCC_STRETCH(512, 32);
-    MCC_STRETCH(1024, 32);
-#undef MCC_STRETCH
+    hipLaunchKernelGGL((token_log_probs_kernel<T, 1024, 32, TOP, false>), dim3((unsigned)(a.rows * c.segments)), dim3(1024),
+                       0, stream, a, c.segments, c.length, stats, best);
     return hipGetLastError();
 }
 
 template <typename T>
 hipError_t forward(hipStream_t stream, const TokenLogProbs& a, void* workspace) {
-    const RowCut c = cut_rows(a.rows, a.vocab);
+    const RowCut c = cut_rows(a.vocab);
     const bool top = a.top > 0 && (a.top_ids || a.top_log_probs);
-    if (c.segments == 1)
-        return top ? launch_stretches<T, true, true>(stream, a, c, nullptr, nullptr)
-                   : launch_stretches<T, false, true>(stream, a, c, nullptr, nullptr);
+    if (c.segments == 1) return top ? launch_rows<T, true>(stream, a, c) : launch_rows<T, false>(stream, a, c);
     SoftmaxStats* stats = static_cast<SoftmaxStats*>(workspace);
     uint64_t* best = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + stats_nbytes(a.rows, c));
-    const hipError_t e = top ? launch_stretches<T, true, false>(stream, a, c, stats, best)
-                             : launch_stretches<T, false, false>(stream, a, c, stats, best);
+    const hipError_t e = top ? launch_stretches<T, true>(stream, a, c, stats, best)
+                             : launch_stretches<T, false>(stream, a, c, stats, best);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(token_log_probs_join_kernel<T>, dim3((unsigned)a.rows), dim3(kJoinThreads), 0, stream, a, c.segments,
                        stats, best);
@@ -426,8 +486,8 @@ hipError_t backward(hipStream_t stream, const void* logits, size_t stride, const
 
 }  // namespace
 
-size_t token_log_probs_workspace_nbytes(ElementType, size_t rows, int vocab, int top) {
-    const RowCut c = cut_rows(rows, vocab);
+size_t token_log_probs_workspace_nbytes(size_t rows, int vocab, int top) {
+    const RowCut c = cut_rows(vocab);
     if (c.segments == 1) return 0;
     return stats_nbytes(rows, c) + rows * c.segments * (size_t)top * sizeof(uint64_t);
 }
@@ -442,13 +502,13 @@ hipError_t launch_token_log_probs(hipStream_t stream, ElementType type, const To
 }
 
 hipError_t launch_softmax_stats(hipStream_t stream, ElementType type, const void* logits, size_t stride, size_t rows,
-                                int vocab, float inv_temperature, const RowCut& cut, SoftmaxStats* stats) {
+                                int vocab, float log2_scale, const RowCut& cut, SoftmaxStats* stats) {
     TokenLogProbs a{};
-    a.logits = logits, a.stride = stride, a.rows = rows, a.vocab = vocab, a.inv_temperature = inv_temperature;
+    a.logits = logits, a.stride = stride, a.rows = rows, a.vocab = vocab, a.log2_scale = log2_scale;
     switch (type) {
-        case ElementType::F32: return launch_stretches<float, false, false>(stream, a, cut, stats, nullptr);
-        case ElementType::F16: return launch_stretches<_Float16, false, false>(stream, a, cut, stats, nullptr);
-        case ElementType::BF16: return launch_stretches<__bf16, false, false>(stream, a, cut, stats, nullptr);
+        case ElementType::F32: return launch_stretches<float, false>(stream, a, cut, stats, nullptr);
+        case ElementType::F16: return launch_stretches<_Float16, false>(stream, a, cut, stats, nullptr);
+        case ElementType::BF16: return launch_stretches<__bf16, false>(stream, a, cut, stats, nullptr);
     }
     return hipErrorInvalidValue;
 }

@@ -224,17 +224,17 @@ def _rows(t, name):
     element = _ELEMENTS.get(t.dtype)
     if element is None:
         raise ValueError("%s: expected float32, float16 or bfloat16, got %s" % (name, t.dtype))
-    if t.dim() == 0:
+    dims = t.dim()
+    if dims == 0:
         raise ValueError("%s: expected at least one dimension" % name)
-    cols = t.shape[-1]
-    rows = t.numel() // cols if cols else 0
-    stride = cols
+    shape = t.shape
+    cols = stride = shape[-1]
+    rows = shape[0] if dims == 2 else t.numel() // cols if cols else 0
     if not t.is_contiguous():
-        if t.dim() != 2 or (t.stride(1) != 1 and cols != 1):
+        if dims != 2 or (t.stride(1) != 1 and cols != 1):
             raise ValueError("%s: expected a contiguous tensor or a matrix with contiguous rows" % name)
         stride = t.stride(0)
-    size = 4 if element == 0 else 2
-    nbytes = ((rows - 1) * stride + cols) * size if rows else 0
+    nbytes = ((rows - 1) * stride + cols) * (2 if element else 4) if rows else 0
     return (t.data_ptr(), nbytes, stride), rows, cols, element
 
 
@@ -243,6 +243,18 @@ def _same_rows(t, like, name):
     if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
         raise ValueError("%s: expected shape %s, %s on %s" % (name, tuple(like.shape), like.dtype, like.device))
     return _rows(t, name)[0]
+
+
+def _out_rows(out, like, buf):
+    """An output with the shape, type and device of `like`, whose _rows() gave `buf`: the caller's tensor or a new
+    one; and its (pointer, bytes, row stride)."""
+    if out is not None:
+        return out, _same_rows(out, like, "out")
+    if not like.is_contiguous():
+        out = like.new_empty(like.shape)
+        return out, _rows(out, "out")[0]
+    out = torch.empty_like(like)
+    return out, (out.data_ptr(), buf[1], buf[2])
 
 
 def _numbers(t, dtype, shape, like, name):
@@ -255,15 +267,26 @@ def _numbers(t, dtype, shape, like, name):
     return _buf(t, dtype)
 
 
+def _new(like, shape, dtype=torch.float32):
+    return like.new_empty(shape, dtype=dtype)
+
+
+# The current stream's handle without a Stream object around it, a tenth of the time; torch's own code
+# generators launch through it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(fn, like, *args):
     """One call on the current stream of the device that `like` is on."""
-    device = like.device
-    stream = torch.cuda.current_stream(device).cuda_stream or None
-    if device.index == torch.cuda.current_device():
-        _lib.check(fn(stream, *args))
+    index = like.get_device()
+    if index == torch.cuda.current_device():
+        rc = fn(_raw_stream(index) or None, *args)
     else:
-        with torch.cuda.device(device):
-            _lib.check(fn(stream, *args))
+        with torch.cuda.device(index):
+            rc = fn(_raw_stream(index) or None, *args)
+    if rc != 0:
+        _lib.check(rc)
 
 
 def _lent(nbytes, workspace, like):
@@ -271,8 +294,9 @@ def _lent(nbytes, workspace, like):
     if workspace is None:
         if nbytes == 0:
             return (None, 0), None
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
-    elif workspace.device != like.device:
+        workspace = _new(like, nbytes, torch.uint8)
+        return (workspace.data_ptr(), nbytes), workspace
+    if workspace.device != like.device:
         raise ValueError("workspace: expected a tensor on %s" % like.device)
     return _buf(workspace, torch.uint8), workspace
 
@@ -281,11 +305,11 @@ def layer_norm(x, gain=None, bias=None, eps=1e-5, out=None):
     """Layer norm of the rows (last dimension) of x: (y, mean, rstd).  gain and bias are float32 vectors;
     `out` may be x."""
     buf, rows, cols, element = _rows(x, "x")
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    y, y_buf = _out_rows(out, x, buf)
+    shape = x.shape[:-1]
+    mean, rstd = _new(x, shape), _new(x, shape)
     _call(_lib.load().mcc_layer_norm, x, *buf, *_numbers(gain, torch.float32, (cols,), x, "gain"),
-          *_numbers(bias, torch.float32, (cols,), x, "bias"), *_same_rows(y, x, "out"),
+          *_numbers(bias, torch.float32, (cols,), x, "bias"), *y_buf,
           mean.data_ptr(), 4 * rows, rstd.data_ptr(), 4 * rows, rows, cols, element, eps)
     return y, mean, rstd
 
@@ -300,18 +324,16 @@ def layer_norm_backward(grad_out, x, mean, rstd, gain=None, bias=True, input_gra
     L = _lib.load()
     buf, rows, cols, element = _rows(x, "x")
     grad_buf = _same_rows(grad_out, x, "grad_out")
-    grad_x = None
-    if input_grad:
-        grad_x = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
-    x_out = _same_rows(grad_x, x, "out") if input_grad else (None, 0, 0)
-    grad_gain = torch.empty(cols, dtype=torch.float32, device=x.device) if gain is not None else None
-    grad_bias = torch.empty(cols, dtype=torch.float32, device=x.device) if bias else None
+    grad_x, x_out = _out_rows(out, x, buf) if input_grad else (None, (None, 0, 0))
+    grad_gain = _new(x, cols) if gain is not None else None
+    grad_bias = _new(x, cols) if bias else None
+    shape, n = x.shape[:-1], 4 * cols
     need = 0 if grad_gain is None and grad_bias is None else L.mcc_layer_norm_backward_workspace_nbytes(rows, cols, element)
     lent, workspace = _lent(need, workspace, x)
-    _call(L.mcc_layer_norm_backward, x, *grad_buf, *buf, *_numbers(mean, torch.float32, x.shape[:-1], x, "mean"),
-          *_numbers(rstd, torch.float32, x.shape[:-1], x, "rstd"), *_numbers(gain, torch.float32, (cols,), x, "gain"),
-          *x_out, *_numbers(grad_gain, torch.float32, (cols,), x, "grad_gain"),
-          *_numbers(grad_bias, torch.float32, (cols,), x, "grad_bias"), *lent, rows, cols, element)
+    _call(L.mcc_layer_norm_backward, x, *grad_buf, *buf, *_numbers(mean, torch.float32, shape, x, "mean"),
+          *_numbers(rstd, torch.float32, shape, x, "rstd"), *_numbers(gain, torch.float32, (cols,), x, "gain"), *x_out,
+          None if grad_gain is None else grad_gain.data_ptr(), n, None if grad_bias is None else grad_bias.data_ptr(), n,
+          *lent, rows, cols, element)
     return grad_x, grad_gain, grad_bias
 
 
@@ -325,15 +347,13 @@ def token_log_probs(logits, tokens=None, top=0, temperature=1.0, workspace=None)
     exponentials, and the `top` likeliest tokens with their log probabilities (None without)."""
     L = _lib.load()
     buf, rows, vocab, element = _rows(logits, "logits")
-    shape, device = logits.shape[:-1], logits.device
+    shape = logits.shape[:-1]
     token_buf = _numbers(tokens, torch.int32, shape, logits, "tokens")
-    log_prob = torch.empty(shape, dtype=torch.float32, device=device) if tokens is not None else None
-    entropy = torch.empty(shape, dtype=torch.float32, device=device)
-    lse = torch.empty(shape, dtype=torch.float32, device=device)
+    log_prob = _new(logits, shape) if tokens is not None else None
+    entropy, lse = _new(logits, shape), _new(logits, shape)
     ids = best = None
     if 0 < top <= MOST_TOP:
-        ids = torch.empty((*shape, top), dtype=torch.int32, device=device)
-        best = torch.empty((*shape, top), dtype=torch.float32, device=device)
+        ids, best = _new(logits, (*shape, top), torch.int32), _new(logits, (*shape, top))
     lent, workspace = _lent(L.mcc_token_log_probs_workspace_nbytes(rows, vocab, top, element) if top >= 0 else 0,
                             workspace, logits)
     n = 4 * rows
@@ -348,13 +368,13 @@ def token_log_probs_backward(logits, tokens, lse, entropy, grad_log_prob, grad_e
     """Gradient of the logits from the gradients of token_log_probs' log_prob and entropy (either may be None);
     lse and entropy are its results.  `out` may be logits."""
     buf, rows, vocab, element = _rows(logits, "logits")
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if out is None else out
+    grad, grad_buf = _out_rows(out, logits, buf)
     shape = logits.shape[:-1]
     f32 = torch.float32
     _call(_lib.load().mcc_token_log_probs_backward, logits, *buf, *_numbers(tokens, torch.int32, shape, logits, "tokens"),
           *_numbers(lse, f32, shape, logits, "lse"), *_numbers(entropy, f32, shape, logits, "entropy"),
           *_numbers(grad_log_prob, f32, shape, logits, "grad_log_prob"),
-          *_numbers(grad_entropy, f32, shape, logits, "grad_entropy"), *_same_rows(grad, logits, "out"),
+          *_numbers(grad_entropy, f32, shape, logits, "grad_entropy"), *grad_buf,
           rows, vocab, element, temperature)
     return grad
 
@@ -370,15 +390,12 @@ def distill_top(logits, teacher_ids, teacher_logits, temperature=1.0, weight=Non
     128; `out` takes grad_logits and may be logits."""
     L = _lib.load()
     buf, rows, vocab, element = _rows(logits, "logits")
-    shape, device = logits.shape[:-1], logits.device
+    shape = logits.shape[:-1]
     if teacher_ids.dim() == 0:
         raise ValueError("teacher_ids: expected [..., entries]")
     top = teacher_ids.shape[-1]
-    loss = torch.empty(shape, dtype=torch.float32, device=device)
-    grad_logits = None
-    if grad:
-        grad_logits = torch.empty(logits.shape, dtype=logits.dtype, device=device) if out is None else out
-    grad_buf = _same_rows(grad_logits, logits, "out") if grad else (None, 0, 0)
+    loss = _new(logits, shape)
+    grad_logits, grad_buf = _out_rows(out, logits, buf) if grad else (None, (None, 0, 0))
     lent, workspace = _lent(L.mcc_distill_top_workspace_nbytes(rows, vocab, element), workspace, logits)
     _call(L.mcc_distill_top, logits, *buf, *_numbers(teacher_ids, torch.int32, (*shape, top), logits, "teacher_ids"),
           *_numbers(teacher_logits, torch.float32, (*shape, top), logits, "teacher_logits"),

@@ -80,9 +80,9 @@ def log_probs(L, z=P, zn=4 * 400, zs=100, tok=2 * P, tokn=16, lp=3 * P, lpn=16, 
     (dict(tokn=15), "tokens buffer"), (dict(tok=P + 1), "tokens must be"), (dict(lpn=15), "log_prob buffer"),
     (dict(hn=15), "entropy buffer"), (dict(lsen=0), "lse buffer"), (dict(idsn=79), "top_ids buffer"),
     (dict(bestn=79), "top_log_probs buffer"),
-    (dict(vocab=9000, zs=9000, zn=4 * 36000), "null"),
-    (dict(vocab=9000, zs=9000, zn=4 * 36000, ws=P + 4, wsn=BIG), "16-byte"),
-    (dict(vocab=9000, zs=9000, zn=4 * 36000, ws=P, wsn=100), "workspace is too small"),
+    (dict(vocab=40000, zs=40000, zn=4 * 160000), "null"),
+    (dict(vocab=40000, zs=40000, zn=4 * 160000, ws=P + 4, wsn=BIG), "16-byte"),
+    (dict(vocab=40000, zs=40000, zn=4 * 160000, ws=P, wsn=100), "workspace is too small"),
     (dict(rows=1 << 30, vocab=1 << 20, zs=1 << 20, zn=1 << 63), "what one call takes"),
 ])
 def test_token_log_probs_refuses(L, kwargs, needle):
@@ -116,8 +116,8 @@ def distill(L, z=P, zn=1600, zs=100, ids=2 * P, idsn=80, y=3 * P, yn=80, w=None,
     (dict(t=-2.0), "temperature"), (dict(t=1e30), "square"), (dict(z=None), "null"), (dict(ids=None), "null"), (dict(y=None), "null"),
     (dict(idsn=79), "teacher_ids buffer"), (dict(yn=79), "teacher_logits buffer"), (dict(w=P, wn=15), "weight buffer"),
     (dict(lossn=15), "loss buffer"), (dict(loss=None, out=None), "no output"), (dict(outn=100), "grad_logits buffer"),
-    (dict(out=P + 4), "overlaps logits"), (dict(vocab=9000, zs=9000, zn=144000, outs=9000, outn=144000), "null"),
-    (dict(vocab=9000, zs=9000, zn=144000, outs=9000, outn=144000, ws=P, wsn=1), "workspace is too small"),
+    (dict(out=P + 4), "overlaps logits"), (dict(vocab=40000, zs=40000, zn=640000, outs=40000, outn=640000), "null"),
+    (dict(vocab=40000, zs=40000, zn=640000, outs=40000, outn=640000, ws=P, wsn=1), "workspace is too small"),
 ])
 def test_distill_top_refuses(L, kwargs, needle):
     refused(L, distill(L, **kwargs), needle)
@@ -125,9 +125,9 @@ def test_distill_top_refuses(L, kwargs, needle):
 
 def test_workspace_sizes(L):
     assert L.mcc_token_log_probs_workspace_nbytes(4, 100, 5, F32) == 0
-    assert L.mcc_token_log_probs_workspace_nbytes(4, 9000, 5, F32) > 0
-    assert L.mcc_token_log_probs_workspace_nbytes(4, 9000, 129, F32) == 0
-    assert L.mcc_token_log_probs_workspace_nbytes(0, 9000, 5, F32) == 0
+    assert L.mcc_token_log_probs_workspace_nbytes(4, 40000, 5, F32) > 0
+    assert L.mcc_token_log_probs_workspace_nbytes(4, 40000, 129, F32) == 0
+    assert L.mcc_token_log_probs_workspace_nbytes(0, 40000, 5, F32) == 0
     assert L.mcc_distill_top_workspace_nbytes(1, 40000, BF16) > 0
     assert L.mcc_distill_top_workspace_nbytes(1, 40000, 17) == 0
     assert L.mcc_layer_norm_backward_workspace_nbytes(1, 64, F32) == 0
