@@ -429,7 +429,10 @@ int mcc_token_log_probs(void* stream, const void* logits, size_t logits_nbytes, 
  *   ((token == j) - p_j) * grad_log_prob - p_j (log p_j + entropy) * grad_entropy,  over temperature.
  * With grad_log_prob = -1 / n it is the gradient of the mean cross entropy.  Ignored positions take no
  * grad_log_prob.  Rows whose upstream gradients are zero and rows of -inf alone get zeros whatever their
- * logits hold.  grad_logits may replace logits.
+ * logits hold.  p is taken as exp(logit / temperature - lse), so lse has to hold it: in a row whose
+ * largest logit is so far from zero that its lse rounds log sum away (beyond 2^24, as the type's lowest
+ * value used as a mask for the whole row) the gradient is not that of the uniform row.  grad_logits may
+ * replace logits.
  */
 int mcc_token_log_probs_backward(void* stream, const void* logits, size_t logits_nbytes, size_t logits_stride,
                                  const int32_t* tokens, size_t tokens_nbytes, const float* lse, size_t lse_nbytes,
@@ -450,13 +453,11 @@ int mcc_token_log_probs_backward(void* stream, const void* logits, size_t logits
  * loss 0 and gradient 0, rows with weight 0 gradient 0 whatever their logits hold; a row of -inf alone has
  * loss +inf and gradient 0.  grad_logits may replace logits.
  */
-size_t mcc_distill_top_workspace_nbytes(size_t rows, size_t vocab, int element);
 int mcc_distill_top(void* stream, const void* logits, size_t logits_nbytes, size_t logits_stride,
                     const int32_t* teacher_ids, size_t teacher_ids_nbytes, const float* teacher_logits,
                     size_t teacher_logits_nbytes, const float* weight, size_t weight_nbytes, float* loss,
                     size_t loss_nbytes, void* grad_logits, size_t grad_logits_nbytes, size_t grad_logits_stride,
-                    void* workspace, size_t workspace_nbytes, size_t rows, size_t vocab, size_t top, int element,
-                    float temperature);
+                    size_t rows, size_t vocab, size_t top, int element, float temperature);
 
 /*
  * Device-resident storage.  Replaces the pooled VulkanRuntime::create_buffer /

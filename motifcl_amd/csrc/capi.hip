@@ -1068,37 +1068,27 @@ int mcc_token_log_probs_backward(void* stream, const void* logits, size_t logits
     return MCC_OK;
 }
 
-size_t mcc_distill_top_workspace_nbytes(size_t rows, size_t vocab, int element) {
-    RowsCheck c{"distill_top", rows, vocab};
-    if (!c.shape(element) || !c.groups(most_stretches(vocab))) return 0;
-    return mcc::distill_top_workspace_nbytes(rows, (int)vocab);
-}
-
 int mcc_distill_top(void* stream, const void* logits, size_t logits_nbytes, size_t logits_stride,
                     const int32_t* teacher_ids, size_t teacher_ids_nbytes, const float* teacher_logits,
                     size_t teacher_logits_nbytes, const float* weight, size_t weight_nbytes, float* loss,
                     size_t loss_nbytes, void* grad_logits, size_t grad_logits_nbytes, size_t grad_logits_stride,
-                    void* workspace, size_t workspace_nbytes, size_t rows, size_t vocab, size_t top, int element,
-                    float temperature) {
+                    size_t rows, size_t vocab, size_t top, int element, float temperature) {
     RowsCheck c{"distill_top", rows, vocab};
     const RowsArg la{logits, logits_nbytes, logits_stride}, ga{grad_logits, grad_logits_nbytes, grad_logits_stride};
     if (!c.shape(element) || !c.temperature(temperature)) return MCC_E_INVALID;
     if (top == 0 || top > MCC_MOST_TOP) return fail(MCC_E_INVALID, "distill_top takes 1 to 128 of a teacher's logits a row");
     if (!std::isfinite(temperature * temperature))
         return fail(MCC_E_INVALID, "distill_top requires a temperature whose square is finite");
-    if (!c.groups(most_stretches(vocab)) || !c.tensor("logits", la) ||
-        !c.numbers("teacher_ids", teacher_ids, teacher_ids_nbytes, rows * top, false) ||
+    if (!c.tensor("logits", la) || !c.numbers("teacher_ids", teacher_ids, teacher_ids_nbytes, rows * top, false) ||
         !c.numbers("teacher_logits", teacher_logits, teacher_logits_nbytes, rows * top, false) ||
         !c.numbers("weight", weight, weight_nbytes, rows, true) || !c.numbers("loss", loss, loss_nbytes, rows, true))
         return MCC_E_INVALID;
     if (grad_logits && (!c.tensor("grad_logits", ga) || !c.apart("grad_logits", ga, "logits", la))) return MCC_E_INVALID;
     if (!loss && !grad_logits) return fail(MCC_E_INVALID, "distill_top received no output");
-    if (!c.workspace(workspace, workspace_nbytes, mcc::distill_top_workspace_nbytes(rows, (int)vocab)))
-        return MCC_E_INVALID;
     const mcc::DistillTop a{logits, logits_stride, rows, (int)vocab, (int)top, temperature, 1.0f / temperature,
                             log2_scale(temperature), teacher_ids, teacher_logits, weight, loss, grad_logits, grad_logits_stride};
     ScopedKernelTimer timer("distill_top", static_cast<hipStream_t>(stream));
-    const hipError_t e = mcc::launch_distill_top(static_cast<hipStream_t>(stream), c.type, a, workspace);
+    const hipError_t e = mcc::launch_distill_top(static_cast<hipStream_t>(stream), c.type, a);
     if (e != hipSuccess) return hip_fail(e, "distill_top launch failed");
     return MCC_OK;
 }

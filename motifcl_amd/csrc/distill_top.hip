@@ -1,12 +1,11 @@
 // Distillation from a teacher's top logits.  With p = softmax(z / T) over the student's whole
 // vocabulary and q = softmax(y / T) over the teacher's entries (id, y) of the row,
 //     loss = T^2 sum q_i (log q_i - log p_id(i)),   d(weight loss)/dz_j = weight T (p_j sum q - sum over id(i) = j of q_i)
-// sum q is 1, or 0 in a row without entries.  Bound by memory: the logits are read once and the gradient
-// is written once.  A workgroup that holds its row in registers does both in one launch; longer rows
-// are cut into stretches: statistics of the stretches, then the rows'
-// losses, then the gradient from a second read.  The teacher's entries change `top` elements of a row: the
-// gradient is written without them first and those elements are written again by the same workgroup
-// behind a barrier, each by the first of the entries that name it.
+// sum q is 1, or 0 in a row without entries.  One workgroup a row, one launch.  Bound by memory: the logits are
+// read once and the gradient is written once where the workgroup's registers hold the row; a longer row is read a
+// second time, as far as the registers and caches do not hold it.  The teacher's entries change `top` elements of a
+// row: the gradient is written without them first and those elements are written again behind a barrier, each by
+// the first of the entries that name it.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -26,9 +25,8 @@ struct Entries {
     float q[kHeld], log_q[kHeld];
     float sum;                    // of q: 1, 0 without entries, NaN where the teacher has no distribution
 };
-// The logits of the entries in [from, from + n) alone are read.
 template <typename T>
-__device__ __forceinline__ Entries load_entries(const DistillTop& a, size_t row, int from, int n, int lane) {
+__device__ __forceinline__ Entries load_entries(const DistillTop& a, size_t row, int lane) {
     Entries e;
     const T* logits = static_cast<const T*>(a.logits) + row * a.stride;
 #pragma unroll
@@ -39,7 +37,7 @@ __device__ __forceinline__ Entries load_entries(const DistillTop& a, size_t row,
         if (e.id[i] < 0 || e.id[i] >= a.vocab) e.id[i] = -1, e.y[i] = -__builtin_inff();
     }
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) e.z[i] = e.id[i] >= from && e.id[i] - from < n ? (float)logits[e.id[i]] : 0.0f;
+    for (int i = 0; i < kHeld; ++i) e.z[i] = e.id[i] >= 0 ? (float)logits[e.id[i]] : 0.0f;
     return e;
 }
 __device__ __forceinline__ void weigh_entries(const DistillTop& a, Entries& e) {
@@ -63,60 +61,71 @@ __device__ __forceinline__ void weigh_entries(const DistillTop& a, Entries& e) {
     }
     e.sum = sum == 0.0f ? 0.0f : sum * inv;
 }
-// T^2 sum q (log q - log p), in every lane of the first wave
-__device__ __forceinline__ float loss_of(const DistillTop& a, const Entries& e, float m, float s) {
-    const float log_s = logf(s);
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-        const float log_p = s == 0.0f ? -__builtin_inff() : (e.z[i] - m) * a.inv_temperature - log_s;
-        if (e.id[i] >= 0 && e.q[i] != 0.0f) sum += e.q[i] * (e.log_q[i] - log_p);
-    }
-    return a.temperature * a.temperature * wave_reduce<Sum>(sum);
-}
-
-// The entries for the patch.  Writing z here also waits for the load of z, so that behind a barrier
-// the logits may be replaced by the gradient.
-struct PatchScratch {
+// The entries in LDS.  Writing z here also waits for the load of z, so that behind a barrier the logits may
+// be replaced by the gradient.
+struct EntryScratch {
     int id[kMostTop];
-    float q[kMostTop], z[kMostTop];
+    float q[kMostTop], log_q[kMostTop], z[kMostTop];
     float sum;
     __device__ __forceinline__ void put(const Entries& e, int lane) {
 #pragma unroll
         for (int i = 0; i < kHeld; ++i) {
             id[lane + 64 * i] = e.id[i];
             q[lane + 64 * i] = e.q[i];
+            log_q[lane + 64 * i] = e.log_q[i];
             z[lane + 64 * i] = e.z[i];
         }
         if (lane == 0) sum = e.sum;
     }
 };
 
-// Gradient of a stretch whose logits are in registers: v = c 2^((z - m) k), and the teacher's entries in
-// it once more, by the first wave.  A barrier lies between lds.put() and this.
+// T^2 sum q (log q - log p), in every lane of the first wave
+__device__ __forceinline__ float loss_of(const DistillTop& a, const EntryScratch& e, float m, float s, int lane) {
+    const float log_s = logf(s);
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = lane; i < kMostTop; i += 64) {
+        const float log_p = s == 0.0f ? -__builtin_inff() : (e.z[i] - m) * a.inv_temperature - log_s;
+        if (e.id[i] >= 0 && e.q[i] != 0.0f) sum += e.q[i] * (e.log_q[i] - log_p);
+    }
+    return a.temperature * a.temperature * wave_reduce<Sum>(sum);
+}
+
+// The gradient without the teacher's entries is c 2^((z - base) k).
+struct GradientScale {
+    float c, scale, base, log2_scale;
+    bool zero;  // rows without weight or without entries, and rows of -inf alone, learn nothing
+    __device__ __forceinline__ GradientScale(const DistillTop& a, size_t row, float m, float s, float sum_q) {
+        const float weight = a.weight ? a.weight[row] : 1.0f;
+        scale = weight * a.temperature;
+        base = shift_of(m);
+        log2_scale = a.log2_scale;
+        zero = weight == 0.0f || sum_q == 0.0f || s == 0.0f;
+        c = scale * sum_q / s;
+    }
+    __device__ __forceinline__ float at(float z) const { return zero ? 0.0f : c * exp2_of((z - base) * log2_scale); }
+};
 template <typename T, int THREADS, int ITERS>
-__device__ __forceinline__ void write_gradient(const DistillTop& a, size_t row, int from, int n,
-                                               const RowVectors<T, THREADS, ITERS>& r, float m, float s,
-                                               const PatchScratch& lds, int t) {
+__device__ __forceinline__ void write_stretch(const GradientScale& c, T* out, int n, const RowVectors<T, THREADS, ITERS>& r,
+                                              int t) {
     typedef RowVectors<T, THREADS, ITERS> Row;
-    const float weight = a.weight ? a.weight[row] : 1.0f, scale = weight * a.temperature, base = shift_of(m);
-    // rows without weight or without entries, and rows of -inf alone, learn nothing
-    const bool zero = weight == 0.0f || lds.sum == 0.0f || s == 0.0f;
-    const float c = scale * lds.sum / s;
-    T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
 #pragma unroll
     for (int j = 0; j < ITERS; ++j) {
         float v[Row::kVec];
 #pragma unroll
-        for (int k = 0; k < Row::kVec; ++k)
-            v[k] = zero ? 0.0f : c * exp2_of(((float)r.raw[j][k] - base) * a.log2_scale);
-        store_row_vector<T, THREADS, ITERS>(out + from, j, t, n, v);
+        for (int k = 0; k < Row::kVec; ++k) v[k] = c.at((float)r.raw[j][k]);
+        store_row_vector<T, THREADS, ITERS>(out, j, t, n, v);
     }
-    __syncthreads();
-    if (t >= 64 || zero) return;
+}
+// The elements that the teacher's entries name, by the first wave; a barrier lies between the writes of the
+// row and this.
+template <typename T>
+__device__ __forceinline__ void patch_entries(const DistillTop& a, const GradientScale& c, T* out,
+                                              const EntryScratch& lds, int t) {
+    if (t >= 64 || c.zero) return;
     for (int at = t; at < a.top; at += 64) {
         const int id = lds.id[at];
-        if (id < from || id - from >= n) continue;
+        if (id < 0) continue;
         float q = 0.0f;
         bool first = true;
         for (int other = 0; other < a.top; ++other)
@@ -124,7 +133,7 @@ __device__ __forceinline__ void write_gradient(const DistillTop& a, size_t row, 
                 q += lds.q[other];
                 first = first && other >= at;
             }
-        if (first) out[id] = (T)(c * exp2_of((lds.z[at] - base) * a.log2_scale) - scale * q);
+        if (first) out[id] = (T)(c.at(lds.z[at]) - c.scale * q);
     }
 }
 
@@ -134,14 +143,13 @@ __global__ __launch_bounds__(THREADS) void distill_row_kernel(DistillTop a) {
     constexpr int kIters = PER_THREAD / Elements<T>::kVec, kWaves = THREADS / 64;
     typedef RowVectors<T, THREADS, kIters> Row;
     __shared__ float slots[3 * kWaves];
-    __shared__ PatchScratch lds;
+    __shared__ EntryScratch lds;
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63, n = a.vocab;
     const size_t row = blockIdx.x;
     Row r;
     r.load(static_cast<const T*>(a.logits) + row * a.stride, t, n);
-    Entries e{};
     if (wave == 0) {
-        e = load_entries<T>(a, row, 0, n, lane);
+        Entries e = load_entries<T>(a, row, lane);
         weigh_entries(a, e);
         lds.put(e, lane);
     }
@@ -149,61 +157,82 @@ __global__ __launch_bounds__(THREADS) void distill_row_kernel(DistillTop a) {
     float thread_max;
     const SoftmaxStats st = stats_of<Row, kWaves, kIters>(r, a.log2_scale, slots, wave, lane, thread_max);
     if (wave == 0 && a.loss) {
-        const float loss = loss_of(a, e, st.m, st.s);
+        const float loss = loss_of(a, lds, st.m, st.s, lane);
         if (lane == 0) a.loss[row] = loss;
     }
     __syncthreads();
-    if (a.grad) write_gradient<T, THREADS, kIters>(a, row, 0, n, r, st.m, st.s, lds, t);
-}
-
-// Rows cut into stretches.  One wave a row joins the statistics into stats[row * segments] (the gradient
-// reads them there) and writes the loss.
-template <typename T>
-__global__ __launch_bounds__(64) void distill_loss_kernel(DistillTop a, int segments, SoftmaxStats* stats) {
-    const size_t row = blockIdx.x;
-    Entries e = load_entries<T>(a, row, 0, a.vocab, threadIdx.x);
-    SoftmaxStats st = stats[row * segments];
-    for (int i = 1; i < segments; ++i) st = join_stats(st, stats[row * segments + i], a.log2_scale);
-    weigh_entries(a, e);
-    const float loss = loss_of(a, e, st.m, st.s);
-    if (threadIdx.x == 0) {
-        if (a.loss) a.loss[row] = loss;
-        stats[row * segments] = st;
-    }
-}
-template <typename T, int THREADS, int PER_THREAD>
-__global__ __launch_bounds__(THREADS) void distill_gradient_kernel(DistillTop a, int segments, int length,
-                                                                   const SoftmaxStats* stats) {
-    constexpr int kIters = PER_THREAD / Elements<T>::kVec;
-    typedef RowVectors<T, THREADS, kIters> Row;
-    __shared__ PatchScratch lds;
-    const int t = threadIdx.x;
-    const size_t row = blockIdx.x / (unsigned)segments;
-    const int from = (int)(blockIdx.x % (unsigned)segments) * length, n = a.vocab - from < length ? a.vocab - from : length;
-    Row r;
-    r.load(static_cast<const T*>(a.logits) + row * a.stride + from, t, n);
-    if (t < 64) {  // another workgroup may have replaced the logits of the entries outside this stretch
-        Entries e = load_entries<T>(a, row, from, n, t);
-        weigh_entries(a, e);
-        lds.put(e, t);
-    }
-    const SoftmaxStats st = stats[row * segments];
+    if (!a.grad) return;
+    const GradientScale c(a, row, st.m, st.s, lds.sum);
+    T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
+    write_stretch<T, THREADS, kIters>(c, out, n, r, t);
     __syncthreads();
-    write_gradient<T, THREADS, kIters>(a, row, from, n, r, st.m, st.s, lds, t);
+    patch_entries(a, c, out, lds, t);
 }
 
+// A row longer than a workgroup's registers (2048 x 128011 f32: 500 us; stretches of rows in workgroups of their
+// own, in a launch for the statistics, one for the losses and one for the gradient, 566 us): the workgroup sweeps
+// the row in stretches, every thread with a maximum and a sum of its own, joins them, and sweeps back
+// to write the gradient, from the last stretch, which it still holds, to the first.
 template <typename T>
-hipError_t distill(hipStream_t stream, ElementType type, const DistillTop& a, void* workspace) {
+__global__ __launch_bounds__(1024, 8) void distill_sweep_kernel(DistillTop a, int segments, int length) {
+    constexpr int kThreads = 1024, kIters = 32 / Elements<T>::kVec, kWaves = kThreads / 64;
+    typedef RowVectors<T, kThreads, kIters> Row;
+    __shared__ float slots[2 * kWaves];
+    __shared__ EntryScratch lds;
+    const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
+    const size_t row = blockIdx.x;
+    const T* logits = static_cast<const T*>(a.logits) + row * a.stride;
+    if (wave == 0) {
+        Entries e = load_entries<T>(a, row, lane);
+        weigh_entries(a, e);
+        lds.put(e, lane);
+    }
+    Row r;
+    float m = -__builtin_inff(), s = 0.0f;
+    int from = 0, n = 0;
+#pragma unroll 1
+    for (int i = 0; i < segments; ++i) {
+        from = i * length, n = a.vocab - from < length ? a.vocab - from : length;
+        r.template load_as<false>(logits + from, t, n);  // read again below: kept in the caches
+        r.fill_tail(t, n, (T)-__builtin_inff());
+        float largest = m;
+#pragma unroll
+        for (int j = 0; j < kIters; ++j)
+#pragma unroll
+            for (int k = 0; k < Row::kVec; ++k) largest = fmaxf(largest, (float)r.raw[j][k]);
+        const float base = shift_of(largest);
+        if (m != -__builtin_inff()) s *= exp2_of((m - base) * a.log2_scale);
+        m = largest;
+#pragma unroll
+        for (int j = 0; j < kIters; ++j)
+#pragma unroll
+            for (int k = 0; k < Row::kVec; ++k) s += exp2_of(((float)r.raw[j][k] - base) * a.log2_scale);
+    }
+    float all_m[1] = {m}, all_s[1];
+    row_reduce<Max, kWaves>(all_m, slots, wave, lane);
+    all_s[0] = m != -__builtin_inff() ? s * exp2_of((m - shift_of(all_m[0])) * a.log2_scale) : s;
+    row_reduce<Sum, kWaves>(all_s, slots + kWaves, wave, lane);
+    if (wave == 0 && a.loss) {
+        const float loss = loss_of(a, lds, all_m[0], all_s[0], lane);
+        if (lane == 0) a.loss[row] = loss;
+    }
+    if (!a.grad) return;
+    const GradientScale c(a, row, all_m[0], all_s[0], lds.sum);
+    T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
+    for (int i = segments - 1;; --i) {
+        write_stretch<T, kThreads, kIters>(c, out + from, n, r, t);
+        if (i == 0) break;
+        from = (i - 1) * length, n = length;
+        r.template load_as<true>(logits + from, t, n);
+    }
+    __syncthreads();
+    patch_entries(a, c, out, lds, t);
+}
+template <typename T>
+hipError_t distill(hipStream_t stream, const DistillTop& a) {
     const RowCut c = cut_rows(a.vocab);
     if (c.segments > 1) {
-        SoftmaxStats* stats = static_cast<SoftmaxStats*>(workspace);
-        hipError_t e = launch_softmax_stats(stream, type, a.logits, a.stride, a.rows, a.vocab, a.log2_scale, c, stats);
-        if (e != hipSuccess) return e;
-        hipLaunchKernelGGL(distill_loss_kernel<T>, dim3((unsigned)a.rows), dim3(64), 0, stream, a, c.segments, stats);
-        e = hipGetLastError();
-        if (e != hipSuccess || !a.grad) return e;
-        hipLaunchKernelGGL((distill_gradient_kernel<T, 1024, 32>), dim3((unsigned)(a.rows * c.segments)), dim3(1024), 0,
-                           stream, a, c.segments, c.length, stats);
+        hipLaunchKernelGGL(distill_sweep_kernel<T>, dim3((unsigned)a.rows), dim3(1024), 0, stream, a, c.segments, c.length);
         return hipGetLastError();
     }
 #define MCC_DISTILL(THREADS, PER_THREAD)                                                                              \
@@ -221,16 +250,11 @@ hipError_t distill(hipStream_t stream, ElementType type, const DistillTop& a, vo
 
 }  // namespace
 
-size_t distill_top_workspace_nbytes(size_t rows, int vocab) {
-    const RowCut c = cut_rows(vocab);
-    return c.segments == 1 ? 0 : rows * c.segments * sizeof(SoftmaxStats);
-}
-
-hipError_t launch_distill_top(hipStream_t stream, ElementType type, const DistillTop& a, void* workspace) {
+hipError_t launch_distill_top(hipStream_t stream, ElementType type, const DistillTop& a) {
     switch (type) {
-        case ElementType::F32: return distill<float>(stream, type, a, workspace);
-        case ElementType::F16: return distill<_Float16>(stream, type, a, workspace);
-        case ElementType::BF16: return distill<__bf16>(stream, type, a, workspace);
+        case ElementType::F32: return distill<float>(stream, a);
+        case ElementType::F16: return distill<_Float16>(stream, a);
+        case ElementType::BF16: return distill<__bf16>(stream, a);
     }
     return hipErrorInvalidValue;
 }

@@ -200,7 +200,6 @@ struct DistillTop {
     void* grad;
     size_t grad_stride;
 };
-size_t distill_top_workspace_nbytes(size_t rows, int vocab);
-hipError_t launch_distill_top(hipStream_t stream, ElementType type, const DistillTop& a, void* workspace);
+hipError_t launch_distill_top(hipStream_t stream, ElementType type, const DistillTop& a);
 
 }  // namespace mcc

@@ -45,6 +45,7 @@ __device__ __forceinline__ SoftmaxStats stats_of(const ROW& r, float scale, floa
     thread_max = largest[0];
     row_reduce<Max, WAVES>(largest, slots, wave, lane);
     st.m = largest[0];
+    // the difference first: of logits at the type's lowest value, as masks may leave a row, z k overflows
     const float base = shift_of(st.m);
     float sums[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -85,9 +86,5 @@ inline RowCut cut_rows(int vocab) {
     else c.threads = 1024, c.per_thread = 32;
     return c;
 }
-
-// Statistics of every stretch of rows that are cut: stats[row * segments + segment].
-hipError_t launch_softmax_stats(hipStream_t stream, ElementType type, const void* logits, size_t stride, size_t rows,
-                                int vocab, float log2_scale, const RowCut& cut, SoftmaxStats* stats);
 
 }  // namespace mcc

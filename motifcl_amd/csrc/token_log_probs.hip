@@ -46,7 +46,7 @@ struct TopScratch {
     static constexpr int kCandidates = WAVES == 1 ? 256 : 512;
     uint64_t list[kCandidates];
     int rank[kCandidates];
-    uint32_t bound;
+    uint32_t groups[WAVES == 1 ? 1 : 256], bound;
     int count;
     float totals[2][WAVES], least[WAVES];
 };
@@ -60,22 +60,37 @@ __device__ __forceinline__ int total_of(int wave_count, float (&totals)[2][WAVES
     return (int)wave_reduce<Sum>(lane < WAVES ? totals[turn][lane] : 0.0f);  // whole numbers below 2^24
 }
 
-// A number that at least `top` of the workgroup's numbers reach: every wave gives the ceil(top / WAVES)-th
-// largest of its lanes' maxima, rounded down to the leading 20 bits of its key (one compare and one
-// population count a bit, the rest scalar), and the smallest of those is reached by as many lanes of
-// every wave.  lds.bound is all ones before.
+// A number that at least `top` of the workgroup's numbers reach.  The threads' maxima are joined over groups
+// of neighbouring lanes, 256 groups a workgroup (64 for a workgroup of one wave), and the first wave finds the
+// top-th largest of the groups' maxima, each of which is a number of its own, by bisection over the leading 20
+// bits of its key: a compare and a population count a bit.  Of random numbers about 256 ln(256 / (256 - top))
+// reach it: 75 for the top 64.
 template <int WAVES>
-__device__ __forceinline__ float lower_bound_of(float thread_max, int top, TopScratch<WAVES>& lds, int lane) {
-    const int nth = (top + WAVES - 1) / WAVES;
-    const uint32_t mine = key_of(thread_max);
+__device__ __forceinline__ float lower_bound_of(float thread_max, int top, TopScratch<WAVES>& lds, int t, int wave, int lane) {
+    constexpr int kLanes = WAVES > 4 ? WAVES / 4 : 1, kGroups = WAVES * 64 / kLanes, kHeld = kGroups / 64;
+    static_assert(kLanes <= 4, "two steps join four lanes");
+    if (kLanes >= 2) thread_max = dpp_join<Max, 0xB1, 0xf>(thread_max);  // quad_perm: lane ^ 1
+    if (kLanes >= 4) thread_max = dpp_join<Max, 0x4E, 0xf>(thread_max);  // lane ^ 2
     uint32_t bound = 0;
+    if (WAVES > 1) {
+        if (lane % kLanes == 0) lds.groups[t / kLanes] = key_of(thread_max);
+        __syncthreads();
+    }
+    if (wave == 0) {
+        uint32_t held[kHeld];
 #pragma unroll
-    for (int bit = 31; bit >= 12; --bit) {
-        const uint32_t next = bound | 1u << bit;
-        if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(mine >= next)) >= nth) bound = next;
+        for (int i = 0; i < kHeld; ++i) held[i] = WAVES > 1 ? lds.groups[i * 64 + lane] : key_of(thread_max);
+#pragma unroll
+        for (int bit = 31; bit >= 12; --bit) {
+            const uint32_t next = bound | 1u << bit;
+            int reach = 0;
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) reach += __builtin_popcountll(__builtin_amdgcn_ballot_w64(held[i] >= next));
+            if (reach >= top) bound = next;
+        }
+        if (WAVES > 1 && lane == 0) lds.bound = bound;
     }
     if (WAVES > 1) {
-        if (lane == 0) atomicMin(&lds.bound, bound);
         __syncthreads();
         bound = lds.bound;
     }
@@ -184,18 +199,29 @@ __device__ __forceinline__ void select_among_ties(const ROW& r, int n, uint32_t 
 template <typename ROW, int WAVES, int ITERS>
 __device__ __forceinline__ int find_candidates(const ROW& r, int n, uint32_t first_id, int top, float thread_max,
                                                TopScratch<WAVES>& lds, int t, int wave, int lane) {
-    const float bound = lower_bound_of<WAVES>(thread_max, top, lds, lane);
-    if (thread_max >= bound) {
+    const float bound = lower_bound_of<WAVES>(thread_max, top, lds, t, wave, lane);
+    auto push = [&](float z, int j, int k) {
+        const int at = atomicAdd(&lds.count, 1);
+        if (at < lds.kCandidates) lds.list[at] = candidate(z, first_id + ROW::index(j, k, again(t), n));
+    };
+    if (bound > -__builtin_inff()) {  // filled elements do not reach it
+        if (thread_max >= bound) {
+#pragma unroll
+            for (int j = 0; j < ITERS; ++j)
+#pragma unroll
+                for (int k = 0; k < ROW::kVec; ++k) {
+                    const float z = (float)r.raw[j][k];
+                    if (z >= bound) push(z, j, k);
+                }
+        }
+    } else if (n <= lds.kCandidates) {
 #pragma unroll
         for (int j = 0; j < ITERS; ++j) {
             const int u = again(t);
 #pragma unroll
             for (int k = 0; k < ROW::kVec; ++k) {
                 const float z = (float)r.raw[j][k];
-                if (z >= bound && ROW::holds(j, k, u, n)) {
-                    const int at = atomicAdd(&lds.count, 1);
-                    if (at < lds.kCandidates) lds.list[at] = candidate(z, first_id + ROW::index(j, k, u, n));
-                }
+                if (z >= bound && ROW::holds(j, k, u, n)) push(z, j, k);
             }
         }
     }
@@ -206,17 +232,15 @@ __device__ __forceinline__ int find_candidates(const ROW& r, int n, uint32_t fir
     return top;
 }
 
-// rank[i] = how many of the n candidates are likelier than list[i].  All the workgroup's threads count: a
-// candidate is compared with a part of the list by each of `parts` threads.
+// rank[i] += how many of the n candidates are likelier than list[i] (0 before).  All the workgroup's threads
+// count: the list is read in parts, one by each group of a power of two of threads that holds the candidates.
 template <int THREADS>
 __device__ __forceinline__ void rank_candidates(const uint64_t* list, int n, int* rank, int t) {
-    for (int i = t; i < n; i += THREADS) rank[i] = 0;
-    __syncthreads();
-    int parts = 1;
-    while (parts < 16 && 2 * parts * n <= THREADS) parts *= 2;
-    const int width = (n + parts - 1) / parts;
-    for (int at = t; at < n * parts; at += THREADS) {
-        const int i = at % n, from = at / n * width, to = from + width < n ? from + width : n;
+    int bits = 32 - __builtin_clz(n > 1 ? n - 1 : 1);
+    if ((1 << bits) > THREADS) bits = 31 - __builtin_clz(THREADS);
+    const int held = 1 << bits, parts = THREADS >> bits, width = (n + parts - 1) / parts;
+    const int from = (t >> bits) * width, to = from + width < n ? from + width : n;
+    for (int i = t & (held - 1); i < n; i += held) {
         const uint64_t mine = list[i];
         int above = 0;
         for (int k = from; k < to; ++k) above += list[k] > mine ? 1 : 0;
@@ -267,7 +291,10 @@ __global__ __launch_bounds__(THREADS, 8) void token_log_probs_kernel(TokenLogPro
     __shared__ float slots[3 * kWaves];
     __shared__ TopScratch<TOP ? kWaves : 1> lds;
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
-    if (TOP && t == 0) lds.count = 0, lds.bound = ~0u;
+    if constexpr (TOP) {  // a barrier of the statistics lies between this and its use
+        if (t == 0) lds.count = 0;
+        for (int i = t; i < lds.kCandidates; i += THREADS) lds.rank[i] = 0;
+    }
     const size_t row = ONE ? blockIdx.x : blockIdx.x / (unsigned)segments;
     const int segment = ONE ? 0 : (int)(blockIdx.x % (unsigned)segments);
     const int from = segment * length, n = a.vocab - from < length ? a.vocab - from : length;
@@ -337,6 +364,7 @@ __global__ __launch_bounds__(kJoinThreads) void token_log_probs_join_kernel(Toke
     }
     if (lane == 0) bounds[wave] = bound;
     if (t == 0) count = 0;
+    for (int i = t; i < kJoinCandidates; i += kJoinThreads) ranks[i] = 0;
     __syncthreads();
     for (int w = 0; w < kWaves; ++w) bound = bounds[w] < bound ? bounds[w] : bound;
     auto gather = [&](uint64_t from) {
@@ -497,18 +525,6 @@ hipError_t launch_token_log_probs(hipStream_t stream, ElementType type, const To
         case ElementType::F32: return forward<float>(stream, a, workspace);
         case ElementType::F16: return forward<_Float16>(stream, a, workspace);
         case ElementType::BF16: return forward<__bf16>(stream, a, workspace);
-    }
-    return hipErrorInvalidValue;
-}
-
-hipError_t launch_softmax_stats(hipStream_t stream, ElementType type, const void* logits, size_t stride, size_t rows,
-                                int vocab, float log2_scale, const RowCut& cut, SoftmaxStats* stats) {
-    TokenLogProbs a{};
-    a.logits = logits, a.stride = stride, a.rows = rows, a.vocab = vocab, a.log2_scale = log2_scale;
-    switch (type) {
-        case ElementType::F32: return launch_stretches<float, false>(stream, a, cut, stats, nullptr);
-        case ElementType::F16: return launch_stretches<_Float16, false>(stream, a, cut, stats, nullptr);
-        case ElementType::BF16: return launch_stretches<__bf16, false>(stream, a, cut, stats, nullptr);
     }
     return hipErrorInvalidValue;
 }

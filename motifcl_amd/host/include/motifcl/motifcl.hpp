@@ -5,6 +5,8 @@
 #include <motifcl/core/error.hpp>
 #include <motifcl/core/shape.hpp>
 #include <motifcl/nn/compact_counter.hpp>
+#include <motifcl/nn/layer_norm.hpp>
+#include <motifcl/ops/loss.hpp>
 #include <motifcl/ops/matmul.hpp>
 #include <motifcl/ops/optim.hpp>
 #include <motifcl/runtime/backend.hpp>

@@ -51,9 +51,8 @@ SIGNATURES = {
     "mcc_token_log_probs_backward": (
         ctypes.c_int, [_vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _sz, _sz, _sz,
                        ctypes.c_int, _f]),
-    "mcc_distill_top_workspace_nbytes": (_sz, [_sz, _sz, ctypes.c_int]),
     "mcc_distill_top": (
-        ctypes.c_int, [_vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _sz, _vp, _sz,
+        ctypes.c_int, [_vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _sz,
                        _sz, _sz, _sz, ctypes.c_int, _f]),
     "mcc_device_alloc": (ctypes.c_int, [ctypes.POINTER(_vp), _sz]),
     "mcc_device_free": (ctypes.c_int, [_vp]),

@@ -307,7 +307,8 @@ def layer_norm(x, gain=None, bias=None, eps=1e-5, out=None):
     buf, rows, cols, element = _rows(x, "x")
     y, y_buf = _out_rows(out, x, buf)
     shape = x.shape[:-1]
-    mean, rstd = _new(x, shape), _new(x, shape)
+    mean = _new(x, shape)
+    rstd = torch.empty_like(mean)
     _call(_lib.load().mcc_layer_norm, x, *buf, *_numbers(gain, torch.float32, (cols,), x, "gain"),
           *_numbers(bias, torch.float32, (cols,), x, "bias"), *y_buf,
           mean.data_ptr(), 4 * rows, rstd.data_ptr(), 4 * rows, rows, cols, element, eps)
@@ -349,8 +350,9 @@ def token_log_probs(logits, tokens=None, top=0, temperature=1.0, workspace=None)
     buf, rows, vocab, element = _rows(logits, "logits")
     shape = logits.shape[:-1]
     token_buf = _numbers(tokens, torch.int32, shape, logits, "tokens")
-    log_prob = _new(logits, shape) if tokens is not None else None
-    entropy, lse = _new(logits, shape), _new(logits, shape)
+    entropy = _new(logits, shape)
+    lse = torch.empty_like(entropy)
+    log_prob = torch.empty_like(entropy) if tokens is not None else None
     ids = best = None
     if 0 < top <= MOST_TOP:
         ids, best = _new(logits, (*shape, top), torch.int32), _new(logits, (*shape, top))
@@ -379,16 +381,11 @@ def token_log_probs_backward(logits, tokens, lse, entropy, grad_log_prob, grad_e
     return grad
 
 
-def distill_top_workspace_nbytes(rows, vocab, dtype):
-    return int(_lib.load().mcc_distill_top_workspace_nbytes(rows, vocab, _ELEMENTS[dtype]))
-
-
-def distill_top(logits, teacher_ids, teacher_logits, temperature=1.0, weight=None, grad=True, out=None, workspace=None):
+def distill_top(logits, teacher_ids, teacher_logits, temperature=1.0, weight=None, grad=True, out=None):
     """Distillation from a teacher's top logits: (loss, grad_logits).  loss is temperature^2 * KL(teacher || student)
     of each row, grad_logits the gradient of sum(weight * loss) (None with grad=False).  teacher_ids (int32, an id
     outside the vocabulary is no entry) and teacher_logits (float32) hold the same number of entries a row, at most
     128; `out` takes grad_logits and may be logits."""
-    L = _lib.load()
     buf, rows, vocab, element = _rows(logits, "logits")
     shape = logits.shape[:-1]
     if teacher_ids.dim() == 0:
@@ -396,10 +393,9 @@ def distill_top(logits, teacher_ids, teacher_logits, temperature=1.0, weight=Non
     top = teacher_ids.shape[-1]
     loss = _new(logits, shape)
     grad_logits, grad_buf = _out_rows(out, logits, buf) if grad else (None, (None, 0, 0))
-    lent, workspace = _lent(L.mcc_distill_top_workspace_nbytes(rows, vocab, element), workspace, logits)
-    _call(L.mcc_distill_top, logits, *buf, *_numbers(teacher_ids, torch.int32, (*shape, top), logits, "teacher_ids"),
+    _call(_lib.load().mcc_distill_top, logits, *buf, *_numbers(teacher_ids, torch.int32, (*shape, top), logits, "teacher_ids"),
           *_numbers(teacher_logits, torch.float32, (*shape, top), logits, "teacher_logits"),
-          *_numbers(weight, torch.float32, shape, logits, "weight"), loss.data_ptr(), 4 * rows, *grad_buf, *lent,
+          *_numbers(weight, torch.float32, shape, logits, "weight"), loss.data_ptr(), 4 * rows, *grad_buf,
           rows, vocab, top, element, temperature)
     return loss, grad_logits
 

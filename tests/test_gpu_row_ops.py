@@ -246,6 +246,28 @@ def check_lowest(ops, z, tokens, top):
 
 
 @pytest.mark.parametrize("vocab", [5, 600, 5000, 40000])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_of_the_lowest_value_are_uniform(ops, vocab, dtype):
+    # everything masked with the type's lowest value: (z - m) / T is 0 wherever z / T is out of range
+    z = torch.full((3, vocab), torch.finfo(dtype).min, device="cuda", dtype=dtype)
+    tokens = torch.tensor([0, vocab - 1, -1], dtype=torch.int32, device="cuda")
+    for temperature in (0.5, 1.0, 2.0):
+        r = ops.token_log_probs(z, tokens, top=3, temperature=temperature)
+        uniform = torch.full((3,), -math.log(vocab), dtype=torch.float64, device="cuda")
+        rows64.close(r.log_prob[:2], uniform[:2], 1.0, 200, "log_prob")
+        rows64.close(r.entropy, -uniform, 1.0, 300, "entropy")
+        rows64.close(r.top_log_probs, uniform[:, None].expand(3, 3), 1.0, 200, "top_log_probs")
+        assert r.top_ids.tolist() == [[0, 1, 2]] * 3
+        ids = torch.tensor([[0, 1]] * 3, dtype=torch.int32, device="cuda")
+        loss, grad = ops.distill_top(z, ids, torch.zeros(3, 2, device="cuda"), temperature)
+        want = temperature ** 2 * (math.log(vocab) - math.log(2)) + 0 * uniform
+        rows64.close(loss, want, 4.0, 400, "loss")
+        at = torch.full((vocab,), temperature / vocab, dtype=torch.float64, device="cuda")
+        at[:2] -= 0.5 * temperature
+        rows64.close(grad, at.expand(3, vocab), 1.0, 400, "grad")
+
+
+@pytest.mark.parametrize("vocab", [5, 600, 5000, 40000])
 def test_token_log_probs_of_empty_and_invalid_rows(ops, vocab):
     g = generator(vocab)
     inf, nan = math.inf, math.nan
