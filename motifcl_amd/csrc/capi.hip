@@ -956,7 +956,7 @@ struct RowsCheck {
 float log2_scale(float temperature) { return (float)(1.44269504088896340736 / (double)temperature); }
 
 // No kernel cuts rows into stretches shorter than 4096 elements.
-size_t most_stretches(size_t cols) { return (cols + 4095) / 4096; }
+size_t most_stretches(size_t cols) { return (cols + 4095) / 4096 + 1; }
 
 }  // namespace
 
@@ -1014,7 +1014,7 @@ int mcc_layer_norm_backward(void* stream, const void* grad_out, size_t grad_out_
 size_t mcc_token_log_probs_workspace_nbytes(size_t rows, size_t vocab, size_t top, int element) {
     RowsCheck c{"token_log_probs", rows, vocab};
     if (!c.shape(element) || top > MCC_MOST_TOP || top > vocab || !c.groups(most_stretches(vocab))) return 0;
-    return mcc::token_log_probs_workspace_nbytes(rows, (int)vocab, (int)top);
+    return mcc::token_log_probs_workspace_nbytes(c.type, rows, (int)vocab, (int)top);
 }
 
 int mcc_token_log_probs(void* stream, const void* logits, size_t logits_nbytes, size_t logits_stride,
@@ -1032,7 +1032,7 @@ int mcc_token_log_probs(void* stream, const void* logits, size_t logits_nbytes, 
         !c.numbers("entropy", entropy, entropy_nbytes, rows, true) || !c.numbers("lse", lse, lse_nbytes, rows, true) ||
         !c.numbers("top_ids", top_ids, top_ids_nbytes, rows * top, true) ||
         !c.numbers("top_log_probs", top_log_probs, top_log_probs_nbytes, rows * top, true) ||
-        !c.workspace(workspace, workspace_nbytes, mcc::token_log_probs_workspace_nbytes(rows, (int)vocab, (int)top)))
+        !c.workspace(workspace, workspace_nbytes, mcc::token_log_probs_workspace_nbytes(c.type, rows, (int)vocab, (int)top)))
         return MCC_E_INVALID;
     const mcc::TokenLogProbs a{logits, logits_stride, rows, (int)vocab, (int)top, 1.0f / temperature,
                                log2_scale(temperature), tokens, log_prob, entropy, lse, top_ids, top_log_probs};

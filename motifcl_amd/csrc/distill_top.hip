@@ -114,7 +114,7 @@ __device__ __forceinline__ void write_stretch(const GradientScale& c, T* out, in
         float v[Row::kVec];
 #pragma unroll
         for (int k = 0; k < Row::kVec; ++k) v[k] = c.at((float)r.raw[j][k]);
-        store_row_vector<T, THREADS, ITERS>(out, j, t, n, v);
+        r.store(out, j, t, n, v);
     }
 }
 // The elements that the teacher's entries name, by the first wave; a barrier lies between the writes of the
@@ -138,10 +138,10 @@ __device__ __forceinline__ void patch_entries(const DistillTop& a, const Gradien
 }
 
 // The row in one workgroup's registers: loss and gradient in one launch.
-template <typename T, int THREADS, int PER_THREAD>
-__global__ __launch_bounds__(THREADS) void distill_row_kernel(DistillTop a) {
-    constexpr int kIters = PER_THREAD / Elements<T>::kVec, kWaves = THREADS / 64;
-    typedef RowVectors<T, THREADS, kIters> Row;
+template <typename T, int THREADS, int ITERS>
+__global__ __launch_bounds__(THREADS, 8) void distill_row_kernel(DistillTop a) {
+    constexpr int kWaves = THREADS / 64;
+    typedef RowVectors<T, THREADS, ITERS> Row;
     __shared__ float slots[3 * kWaves];
     __shared__ EntryScratch lds;
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63, n = a.vocab;
@@ -155,7 +155,7 @@ __global__ __launch_bounds__(THREADS) void distill_row_kernel(DistillTop a) {
     }
     r.fill_tail(t, n, (T)-__builtin_inff());
     float thread_max;
-    const SoftmaxStats st = stats_of<Row, kWaves, kIters>(r, a.log2_scale, slots, wave, lane, thread_max);
+    const SoftmaxStats st = stats_of<Row, kWaves, ITERS>(r, a.log2_scale, slots, wave, lane, thread_max);
     if (wave == 0 && a.loss) {
         const float loss = loss_of(a, lds, st.m, st.s, lane);
         if (lane == 0) a.loss[row] = loss;
@@ -164,7 +164,7 @@ __global__ __launch_bounds__(THREADS) void distill_row_kernel(DistillTop a) {
     if (!a.grad) return;
     const GradientScale c(a, row, st.m, st.s, lds.sum);
     T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
-    write_stretch<T, THREADS, kIters>(c, out, n, r, t);
+    write_stretch<T, THREADS, ITERS>(c, out, n, r, t);
     __syncthreads();
     patch_entries(a, c, out, lds, t);
 }
@@ -175,7 +175,7 @@ __global__ __launch_bounds__(THREADS) void distill_row_kernel(DistillTop a) {
 // to write the gradient, from the last stretch, which it still holds, to the first.
 template <typename T>
 __global__ __launch_bounds__(1024, 8) void distill_sweep_kernel(DistillTop a, int segments, int length) {
-    constexpr int kThreads = 1024, kIters = 32 / Elements<T>::kVec, kWaves = kThreads / 64;
+    constexpr int kThreads = 1024, kIters = 8, kWaves = kThreads / 64;
     typedef RowVectors<T, kThreads, kIters> Row;
     __shared__ float slots[2 * kWaves];
     __shared__ EntryScratch lds;
@@ -193,13 +193,14 @@ __global__ __launch_bounds__(1024, 8) void distill_sweep_kernel(DistillTop a, in
 #pragma unroll 1
     for (int i = 0; i < segments; ++i) {
         from = i * length, n = a.vocab - from < length ? a.vocab - from : length;
-        r.template load_as<false>(logits + from, t, n);  // read again below: kept in the caches
+        r.template load<false>(logits + from, again(t), n);  // read again below: kept in the caches
         r.fill_tail(t, n, (T)-__builtin_inff());
         float largest = m;
 #pragma unroll
         for (int j = 0; j < kIters; ++j)
 #pragma unroll
             for (int k = 0; k < Row::kVec; ++k) largest = fmaxf(largest, (float)r.raw[j][k]);
+        r.convert_again();
         const float base = shift_of(largest);
         if (m != -__builtin_inff()) s *= exp2_of((m - base) * a.log2_scale);
         m = largest;
@@ -208,6 +209,7 @@ __global__ __launch_bounds__(1024, 8) void distill_sweep_kernel(DistillTop a, in
 #pragma unroll
             for (int k = 0; k < Row::kVec; ++k) s += exp2_of(((float)r.raw[j][k] - base) * a.log2_scale);
     }
+    r.convert_again();
     float all_m[1] = {m}, all_s[1];
     row_reduce<Max, kWaves>(all_m, slots, wave, lane);
     all_s[0] = m != -__builtin_inff() ? s * exp2_of((m - shift_of(all_m[0])) * a.log2_scale) : s;
@@ -219,32 +221,27 @@ __global__ __launch_bounds__(1024, 8) void distill_sweep_kernel(DistillTop a, in
     if (!a.grad) return;
     const GradientScale c(a, row, all_m[0], all_s[0], lds.sum);
     T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
+#pragma unroll 1
     for (int i = segments - 1;; --i) {
-        write_stretch<T, kThreads, kIters>(c, out + from, n, r, t);
+        write_stretch<T, kThreads, kIters>(c, out + from, n, r, again(t));
         if (i == 0) break;
         from = (i - 1) * length, n = length;
-        r.template load_as<true>(logits + from, t, n);
+        r.load(logits + from, again(t), n);
     }
     __syncthreads();
     patch_entries(a, c, out, lds, t);
 }
 template <typename T>
 hipError_t distill(hipStream_t stream, const DistillTop& a) {
-    const RowCut c = cut_rows(a.vocab);
+    const RowCut c = cut_rows(a.vocab, Elements<T>::kVec);
     if (c.segments > 1) {
         hipLaunchKernelGGL(distill_sweep_kernel<T>, dim3((unsigned)a.rows), dim3(1024), 0, stream, a, c.segments, c.length);
         return hipGetLastError();
     }
-#define MCC_DISTILL(THREADS, PER_THREAD)                                                                              \
-    if (c.threads == THREADS && c.per_thread == PER_THREAD)                                                           \
-    hipLaunchKernelGGL((distill_row_kernel<T, THREADS, PER_THREAD>), dim3((unsigned)a.rows), dim3(THREADS), 0, stream, a)
-    MCC_DISTILL(64, 8);
-    MCC_DISTILL(64, 32);
-    MCC_DISTILL(256, 16);
-    MCC_DISTILL(256, 32);
-    MCC_DISTILL(512, 32);
-    MCC_DISTILL(1024, 32);
-#undef MCC_DISTILL
+    for_shape<T>(c, [&](auto threads, auto iters) {
+        constexpr int THREADS = decltype(threads)::value, ITERS = decltype(iters)::value;
+        hipLaunchKernelGGL((distill_row_kernel<T, THREADS, ITERS>), dim3((unsigned)a.rows), dim3(THREADS), 0, stream, a);
+    });
     return hipGetLastError();
 }
 

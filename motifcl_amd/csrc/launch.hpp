@@ -179,7 +179,7 @@ struct TokenLogProbs {
     int32_t* top_ids;
     float* top_log_probs;
 };
-size_t token_log_probs_workspace_nbytes(size_t rows, int vocab, int top);
+size_t token_log_probs_workspace_nbytes(ElementType type, size_t rows, int vocab, int top);
 hipError_t launch_token_log_probs(hipStream_t stream, ElementType type, const TokenLogProbs& a, void* workspace);
 hipError_t launch_token_log_probs_backward(hipStream_t stream, ElementType type, const void* logits, size_t stride,
                                            const int32_t* tokens, const float* lse, const float* entropy,

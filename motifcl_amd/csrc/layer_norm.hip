@@ -19,12 +19,13 @@ namespace {
 
 // The kVec floats of a column vector (gain, bias) that belong to vector j of thread t.
 template <typename ROW>
-__device__ __forceinline__ void load_columns(const float* p, int j, int t, int n, float none, float (&v)[ROW::kVec]) {
+__device__ __forceinline__ void load_columns(const ROW& r, const float* p, int j, int t, int n, float none,
+                                             float (&v)[ROW::kVec]) {
     if (!p) {
 #pragma unroll
         for (int k = 0; k < ROW::kVec; ++k) v[k] = none;
     } else if (n >= ROW::kVec) {
-        const int at = ROW::place(j, t, n);
+        const int at = r.place(j, t, n);
 #pragma unroll
         for (int k = 0; k < ROW::kVec; k += 4) {
             const Elements<float>::Vec q = *reinterpret_cast<const Elements<float>::Vec*>(p + at + k);
@@ -32,13 +33,13 @@ __device__ __forceinline__ void load_columns(const float* p, int j, int t, int n
         }
     } else {
 #pragma unroll
-        for (int k = 0; k < ROW::kVec; ++k) v[k] = ROW::first(j, t) + k < n ? p[ROW::first(j, t) + k] : none;
+        for (int k = 0; k < ROW::kVec; ++k) v[k] = r.holds(j, k, t, n) ? p[r.index(j, k, t, n)] : none;
     }
 }
 
 template <typename ROW>
-__device__ __forceinline__ void store_columns(float* p, int j, int t, int n, const float (&v)[ROW::kVec]) {
-    const int e = ROW::first(j, t);
+__device__ __forceinline__ void store_columns(const ROW& r, float* p, int j, int t, int n, const float (&v)[ROW::kVec]) {
+    const int e = r.first(j, t);
     if (e + ROW::kVec <= n) {
 #pragma unroll
         for (int k = 0; k < ROW::kVec; k += 4) {
@@ -48,14 +49,16 @@ __device__ __forceinline__ void store_columns(float* p, int j, int t, int n, con
     } else {
 #pragma unroll
         for (int k = 0; k < ROW::kVec; ++k)
-            if (ROW::holds(j, k, t, n)) p[ROW::index(j, k, t, n)] = v[k];
+            if (r.holds(j, k, t, n)) p[r.index(j, k, t, n)] = v[k];
     }
 }
 
 __device__ __forceinline__ float inv_sqrt(float x) { return 1.0f / sqrtf(x); }
 
-// THREADS threads hold a row, SLOTS rows share a workgroup (only where a row is one wave's).
-template <typename T, int THREADS, int ITERS, int SLOTS>
+// THREADS threads hold a row, SLOTS rows share a workgroup (only where a row is one wave's), and each of them
+// takes ROWS rows one behind the other, all read at once: gain and bias are then read once for ROWS rows,
+// and a reduction serves them all.
+template <typename T, int THREADS, int ITERS, int SLOTS, int ROWS>
 __global__ __launch_bounds__(THREADS* SLOTS) void layer_norm_kernel(const T* x, size_t x_stride, const float* gain,
                                                                     const float* bias, T* y, size_t y_stride,
                                                                     float* mean_out, float* rstd_out, size_t rows,
@@ -63,44 +66,60 @@ __global__ __launch_bounds__(THREADS* SLOTS) void layer_norm_kernel(const T* x, 
     static_assert(SLOTS == 1 || THREADS == 64, "waves of a shared workgroup leave one by one");
     typedef RowVectors<T, THREADS, ITERS> Row;
     constexpr int kWaves = THREADS / 64;
-    __shared__ float slots[2 * kWaves];
+    __shared__ float slots[2 * ROWS * kWaves];
     const int t = threadIdx.x % THREADS, wave = t >> 6, lane = threadIdx.x & 63;
-    const size_t row = (size_t)blockIdx.x * SLOTS + threadIdx.x / THREADS;
+    const size_t row = ((size_t)blockIdx.x * SLOTS + __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS)) * ROWS;
     if (row >= rows) return;
-    Row r;
-    r.load(x + row * x_stride, t, n);
-    r.fill_tail(t, n, (T)0.0f);
-    float sum[1] = {0.0f};
+    Row r[ROWS];
+    float sum[ROWS], squares[ROWS], mean[ROWS], rstd[ROWS];
 #pragma unroll
-    for (int j = 0; j < ITERS; ++j)
+    for (int i = 0; i < ROWS; ++i) {  // rows behind the last are the last once more
+        r[i].load(x + (row + i < rows ? row + i : rows - 1) * x_stride, t, n);
+        sum[i] = squares[i] = 0.0f;
+    }
 #pragma unroll
-        for (int k = 0; k < Row::kVec; ++k) sum[0] += (float)r.raw[j][k];
+    for (int i = 0; i < ROWS; ++i) {
+        r[i].fill_tail(t, n, (T)0.0f);
+#pragma unroll
+        for (int j = 0; j < ITERS; ++j)
+#pragma unroll
+            for (int k = 0; k < Row::kVec; ++k) sum[i] += (float)r[i].raw[j][k];
+    }
     row_reduce<Sum, kWaves>(sum, slots, wave, lane);
-    const float mean = sum[0] * inv_n;
-    float squares[1] = {0.0f};
 #pragma unroll
-    for (int j = 0; j < ITERS; ++j) {
-        const bool whole = (j + 1) * THREADS * Row::kVec <= n;
+    for (int i = 0; i < ROWS; ++i) {
+        mean[i] = sum[i] * inv_n;
 #pragma unroll
-        for (int k = 0; k < Row::kVec; ++k) {
-            const float d = (float)r.raw[j][k] - mean;
-            if (whole || Row::holds(j, k, t, n)) squares[0] = fmaf(d, d, squares[0]);
+        for (int j = 0; j < ITERS; ++j) {
+            const bool whole = r[i].whole(j, n);
+#pragma unroll
+            for (int k = 0; k < Row::kVec; ++k) {
+                const float d = (float)r[i].raw[j][k] - mean[i];
+                if (whole || r[i].holds(j, k, t, n)) squares[i] = fmaf(d, d, squares[i]);
+            }
         }
     }
-    row_reduce<Sum, kWaves>(squares, slots + kWaves, wave, lane);
-    const float rstd = inv_sqrt(squares[0] * inv_n + eps);
-    if (t == 0) {
-        if (mean_out) mean_out[row] = mean;
-        if (rstd_out) rstd_out[row] = rstd;
+    row_reduce<Sum, kWaves>(squares, slots + ROWS * kWaves, wave, lane);
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        rstd[i] = inv_sqrt(squares[i] * inv_n + eps);
+        if (t == 0 && row + i < rows) {
+            if (mean_out) mean_out[row + i] = mean[i];
+            if (rstd_out) rstd_out[row + i] = rstd[i];
+        }
     }
 #pragma unroll
     for (int j = 0; j < ITERS; ++j) {
-        float g[Row::kVec], b[Row::kVec], v[Row::kVec];
-        load_columns<Row>(gain, j, t, n, 1.0f, g);
-        load_columns<Row>(bias, j, t, n, 0.0f, b);
+        float g[Row::kVec], b[Row::kVec];
+        load_columns(r[0], gain, j, t, n, 1.0f, g);
+        load_columns(r[0], bias, j, t, n, 0.0f, b);
 #pragma unroll
-        for (int k = 0; k < Row::kVec; ++k) v[k] = fmaf(((float)r.raw[j][k] - mean) * rstd, g[k], b[k]);
-        store_row_vector<T, THREADS, ITERS>(y + row * y_stride, j, t, n, v);
+        for (int i = 0; i < ROWS; ++i) {
+            float v[Row::kVec];
+#pragma unroll
+            for (int k = 0; k < Row::kVec; ++k) v[k] = fmaf(((float)r[i].raw[j][k] - mean[i]) * rstd[i], g[k], b[k]);
+            if (row + i < rows) r[i].store(y + (row + i) * y_stride, j, t, n, v);
+        }
     }
 }
 
@@ -138,9 +157,7 @@ __global__ __launch_bounds__(kLongThreads) void layer_norm_long_kernel(const T* 
 // ---- backward -----------------------------------------------------------------------------------
 // A workgroup walks rows blockIdx * SLOTS + slot, + gridDim * SLOTS, ...; every thread keeps its
 // columns' sums.  partial: [gridDim][2][n], the gain's and the bias's sums of the workgroup's rows.
-// STREAM is chosen for all rows at once: loads on two paths would be waited for together in the loop
-// (32768 x 4096 bf16: 173 us instead of 142 us).
-template <typename T, int THREADS, int ITERS, int SLOTS, bool STREAM>
+template <typename T, int THREADS, int ITERS, int SLOTS>
 __global__ __launch_bounds__(THREADS* SLOTS) void layer_norm_backward_kernel(
     const T* grad_out, size_t grad_out_stride, const T* x, size_t x_stride, const float* mean_in, const float* rstd_in,
     const float* gain, T* grad_x, size_t grad_x_stride, float* partial_gain, float* partial_bias, size_t partial_stride,
@@ -152,15 +169,15 @@ __global__ __launch_bounds__(THREADS* SLOTS) void layer_norm_backward_kernel(
     const int t = threadIdx.x % THREADS, slot = threadIdx.x / THREADS, wave = t >> 6, lane = threadIdx.x & 63;
     float dgain[ITERS][Row::kVec] = {}, dbias[ITERS][Row::kVec] = {};
     float g[ITERS][Row::kVec];
+    Row rx, rd;
 #pragma unroll
-    for (int j = 0; j < ITERS; ++j) load_columns<Row>(gain, j, t, n, 1.0f, g[j]);
+    for (int j = 0; j < ITERS; ++j) load_columns(rx, gain, j, t, n, 1.0f, g[j]);
     int turn = 0;
     for (size_t base = (size_t)blockIdx.x * SLOTS; base < rows; base += (size_t)gridDim.x * SLOTS, turn ^= 1) {
         const bool live = base + slot < rows;
         const size_t row = live ? base + slot : rows - 1;
-        Row rx, rd;
-        rx.template load_as<STREAM>(x + row * x_stride, t, n);
-        rd.template load_as<STREAM>(grad_out + row * grad_out_stride, t, n);
+        rx.load(x + row * x_stride, t, n);
+        rd.load(grad_out + row * grad_out_stride, t, n);
         const float mean = mean_in[row], rstd = rstd_in[row];
         rd.fill_tail(t, n, (T)0.0f);  // the sums then need no other mask
         rx.fill_tail(t, n, (T)0.0f);
@@ -189,7 +206,7 @@ __global__ __launch_bounds__(THREADS* SLOTS) void layer_norm_backward_kernel(
                     const float xhat = ((float)rx.raw[j][k] - mean) * rstd;
                     v[k] = rstd * ((float)rd.raw[j][k] * g[j][k] - a - xhat * b);
                 }
-                store_row_vector<T, THREADS, ITERS>(grad_x + row * grad_x_stride, j, t, n, v);
+                rd.store(grad_x + row * grad_x_stride, j, t, n, v);
             }
         }
     }
@@ -218,8 +235,8 @@ __global__ __launch_bounds__(THREADS* SLOTS) void layer_norm_backward_kernel(
     if (slot != 0) return;
 #pragma unroll
     for (int j = 0; j < ITERS; ++j) {
-        if (partial_gain) store_columns<Row>(partial_gain + (size_t)blockIdx.x * partial_stride, j, t, n, dgain[j]);
-        if (partial_bias) store_columns<Row>(partial_bias + (size_t)blockIdx.x * partial_stride, j, t, n, dbias[j]);
+        if (partial_gain) store_columns(rx, partial_gain + (size_t)blockIdx.x * partial_stride, j, t, n, dgain[j]);
+        if (partial_bias) store_columns(rx, partial_bias + (size_t)blockIdx.x * partial_stride, j, t, n, dbias[j]);
     }
 }
 
@@ -320,6 +337,9 @@ size_t backward_groups(size_t rows, int n, int vec) {
     return groups < most ? groups : most;
 }
 
+// Rows from which a wave or workgroup takes several (fewer are spread over the device).
+constexpr size_t kManyRows = 4096;
+
 template <typename T>
 hipError_t forward(hipStream_t stream, const void* xv, size_t x_stride, const float* gain, const float* bias, void* yv,
                    size_t y_stride, float* mean, float* rstd, size_t rows, int n, float eps) {
@@ -328,23 +348,33 @@ hipError_t forward(hipStream_t stream, const void* xv, size_t x_stride, const fl
     const float inv_n = 1.0f / (float)n;
     constexpr int vec = Elements<T>::kVec;
     const int vectors = (n + vec - 1) / vec;
-#define MCC_NORM(THREADS, ITERS, SLOTS)                                                                            \
-    hipLaunchKernelGGL((layer_norm_kernel<T, THREADS, ITERS, SLOTS>), dim3((unsigned)((rows + SLOTS - 1) / SLOTS)), \
-                       dim3(THREADS * SLOTS), 0, stream, x, x_stride, gain, bias, y, y_stride, mean, rstd, rows, n, \
-                       inv_n, eps)
+#define MCC_NORM_AS(THREADS, ITERS, SLOTS, ROWS)                                                                   \
+    hipLaunchKernelGGL((layer_norm_kernel<T, THREADS, ITERS, SLOTS, ROWS>),                                        \
+                       dim3((unsigned)((rows + SLOTS * ROWS - 1) / (SLOTS * ROWS))), dim3(THREADS * SLOTS), 0, stream, \
+                       x, x_stride, gain, bias, y, y_stride, mean, rstd, rows, n, inv_n, eps)
+#define MCC_NORM(THREADS, ITERS, SLOTS, ROWS)                                          \
+    do {                                                                               \
+        if (rows < kManyRows) MCC_NORM_AS(THREADS, ITERS, SLOTS, 1);                   \
+        else MCC_NORM_AS(THREADS, ITERS, SLOTS, ROWS);                                 \
+    } while (0)
+    // Sixteen-bit rows are read with half the bytes of gain and bias to theirs that 32-bit rows need twice: sharing
+    // them pays there (16384 x 4096 bf16: 58 us alone, 53 us by two, 52 us by four; 8191 wide 145 us alone, 112 us by
+    // two), and not for f32 (32768 x 4096: 178 us alone, 188 us by two).
+    constexpr int kRows = vec == 8 ? 4 : 1, kRows4 = vec == 8 ? 2 : 1;
     // a row is a wave's up to 32 elements a thread, then a workgroup's of 256, then of 1024 threads
-    if (vectors <= 64) MCC_NORM(64, 1, 4);
-    else if (vectors <= 128) MCC_NORM(64, 2, 4);
-    else if (vectors <= 256) MCC_NORM(64, 4, 4);
-    else if (vectors <= 512) MCC_NORM(256, 2, 1);
-    else if (vectors <= 1024) MCC_NORM(256, 4, 1);
-    else if (vectors <= 2048) MCC_NORM(256, 8, 1);
-    else if (vectors <= 4096) MCC_NORM(1024, 4, 1);
-    else if (vectors <= 8192) MCC_NORM(1024, 8, 1);
+    if (vectors <= 64) MCC_NORM(64, 1, 4, kRows);
+    else if (vectors <= 128) MCC_NORM(64, 2, 4, kRows);
+    else if (vectors <= 256) MCC_NORM(64, 4, 4, kRows4);
+    else if (vectors <= 512) MCC_NORM(256, 2, 1, kRows);
+    else if (vectors <= 1024) MCC_NORM(256, 4, 1, kRows4);
+    else if (vectors <= 2048) MCC_NORM(512, 4, 1, 1);
+    else if (vectors <= 4096) MCC_NORM(1024, 4, 1, 1);
+    else if (vectors <= 8192) MCC_NORM(1024, 8, 1, 1);
     else
         hipLaunchKernelGGL(layer_norm_long_kernel<T>, dim3((unsigned)rows), dim3(kLongThreads), 0, stream, x, x_stride,
                            gain, bias, y, y_stride, mean, rstd, n, inv_n, eps);
 #undef MCC_NORM
+#undef MCC_NORM_AS
     return hipGetLastError();
 }
 
@@ -362,23 +392,19 @@ hipError_t backward(hipStream_t stream, const void* dv, size_t d_stride, const v
     const size_t stride = join ? 2 * (size_t)n : 0;
     float* pg = !grad_gain ? nullptr : join ? workspace : grad_gain;
     float* pb = !grad_bias ? nullptr : join ? workspace + n : grad_bias;
-    const bool stream_rows = streamed(x) && streamed(d) && x_stride * sizeof(T) % 128 == 0 && d_stride * sizeof(T) % 128 == 0;
-#define MCC_NORM_BACKWARD_AS(THREADS, ITERS, SLOTS, STREAM)                                                            \
-    hipLaunchKernelGGL((layer_norm_backward_kernel<T, THREADS, ITERS, SLOTS, STREAM>), dim3((unsigned)groups),         \
+#define MCC_NORM_BACKWARD(THREADS, ITERS, SLOTS)                                                                     \
+    hipLaunchKernelGGL((layer_norm_backward_kernel<T, THREADS, ITERS, SLOTS>), dim3((unsigned)groups),               \
                        dim3(THREADS * SLOTS), 0, stream, d, d_stride, x, x_stride, mean, rstd, gain, gx, g_stride, pg, \
                        pb, stride, rows, n, inv_n)
-#define MCC_NORM_BACKWARD(THREADS, ITERS, SLOTS)                             \
-    if (stream_rows) MCC_NORM_BACKWARD_AS(THREADS, ITERS, SLOTS, true);      \
-    else MCC_NORM_BACKWARD_AS(THREADS, ITERS, SLOTS, false)
     constexpr int most = vec == 4 ? 4 : 2;
     if (shape.threads == 64) {
-        if (shape.iters == 1) { MCC_NORM_BACKWARD(64, 1, 8); }
-        else if (shape.iters == 2) { MCC_NORM_BACKWARD(64, 2, 8); }
-        else { MCC_NORM_BACKWARD(64, most, 8); }
+        if (shape.iters == 1) MCC_NORM_BACKWARD(64, 1, 8);
+        else if (shape.iters == 2) MCC_NORM_BACKWARD(64, 2, 8);
+        else MCC_NORM_BACKWARD(64, most, 8);
     } else if (shape.threads == 256) {
-        if (shape.iters == 1) { MCC_NORM_BACKWARD(256, 1, 2); }
-        else if (shape.iters == 2) { MCC_NORM_BACKWARD(256, 2, 2); }
-        else { MCC_NORM_BACKWARD(256, most, 2); }
+        if (shape.iters == 1) MCC_NORM_BACKWARD(256, 1, 2);
+        else if (shape.iters == 2) MCC_NORM_BACKWARD(256, 2, 2);
+        else MCC_NORM_BACKWARD(256, most, 2);
     } else if (shape.threads == 512) {
         MCC_NORM_BACKWARD(512, most, 1);
     } else if (shape.threads == 1024) {
@@ -393,7 +419,6 @@ hipError_t backward(hipStream_t stream, const void* dv, size_t d_stride, const v
                                d_stride, x, x_stride, mean, rstd, gain, gx, g_stride, n, inv_n);
     }
 #undef MCC_NORM_BACKWARD
-#undef MCC_NORM_BACKWARD_AS
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !join || (!pg && !pb)) return e;
     hipLaunchKernelGGL(layer_norm_join_kernel, dim3((unsigned)((n + kJoinColumns - 1) / kJoinColumns), 2),

@@ -34,7 +34,7 @@ __device__ __forceinline__ SoftmaxStats join_stats(SoftmaxStats a, SoftmaxStats 
 
 // scale is k above; slots: 3 * WAVES floats of LDS that no wave still reads
 template <typename ROW, int WAVES, int ITERS>
-__device__ __forceinline__ SoftmaxStats stats_of(const ROW& r, float scale, float* slots, int wave, int lane,
+__device__ __forceinline__ SoftmaxStats stats_of(ROW& r, float scale, float* slots, int wave, int lane,
                                                  float& thread_max) {
     SoftmaxStats st;
     float largest[1] = {-__builtin_inff()};
@@ -44,6 +44,7 @@ __device__ __forceinline__ SoftmaxStats stats_of(const ROW& r, float scale, floa
         for (int k = 0; k < ROW::kVec; ++k) largest[0] = fmaxf(largest[0], (float)r.raw[j][k]);
     thread_max = largest[0];
     row_reduce<Max, WAVES>(largest, slots, wave, lane);
+    r.convert_again();
     st.m = largest[0];
     // the difference first: of logits at the type's lowest value, as masks may leave a row, z k overflows
     const float base = shift_of(st.m);
@@ -57,34 +58,56 @@ __device__ __forceinline__ SoftmaxStats stats_of(const ROW& r, float scale, floa
             sums[1] = fmaf(e, fmaxf(d, -1e4f), sums[1]);  // e is 0 long before the bound: 0 * -inf does not arise
         }
     row_reduce<Sum, WAVES>(sums, slots + WAVES, wave, lane);
+    r.convert_again();
     st.s = sums[0];
     st.u = sums[1];
     return st;
 }
 
 // A row of `vocab` numbers is cut into `segments` stretches of `length` numbers (the last may be
-// shorter), each held by a workgroup of `threads` threads, `per_thread` numbers a thread.
+// shorter), each held by a workgroup of `threads` threads, `iters` vectors of `vec` numbers a thread.
 struct RowCut {
-    int threads, per_thread, segments, length;
+    int threads, iters, segments, length;
 };
-constexpr int kMostHeld = 32768;  // numbers in the registers of a workgroup of 1024 threads
-// Rows are cut only where a workgroup cannot hold one.  Cutting few rows further, so that more CUs read
-// them, does not pay for the launch that joins the stretches: one row of 32768 f32 takes 30.7 us from call to
-// end whole and 34.6 us in eight stretches, 200 rows 35 and 39 us, one row of 128011 37 us in four stretches
-// and 45 us in 32.
-inline RowCut cut_rows(int vocab) {
+// Rows are cut only where a workgroup cannot hold one, in at most 32 registers a thread.  Cutting few rows
+// further, so that more CUs read them, does not pay for the launch that joins the stretches: one row of 32768
+// f32 takes 30.7 us from call to end whole and 34.6 us in eight stretches, 200 rows 35 and 39 us.
+// Sixteen-bit rows are bound by the vector units and want few waves, which share the work that is done once a
+// wave (distillation of 4096 x 16384 bf16: 56 us with 512 threads, 72 us with 1024); f32 rows are bound by
+// memory and want many (114 and 103 us).
+inline RowCut cut_rows(int vocab, int vec) {
     RowCut c;
-    c.segments = (int)(((size_t)vocab + kMostHeld - 1) / kMostHeld);
-    const size_t even = ((size_t)vocab + c.segments - 1) / c.segments;
-    c.length = (int)((even + 7) / 8 * 8);  // stretches begin where 16-byte accesses of an aligned row do
-    if (c.segments > 1) c.threads = 1024, c.per_thread = 32;  // longer than half of what it holds
-    else if (vocab <= 512) c.threads = 64, c.per_thread = 8;
-    else if (vocab <= 2048) c.threads = 64, c.per_thread = 32;
-    else if (vocab <= 4096) c.threads = 256, c.per_thread = 16;
-    else if (vocab <= 8192) c.threads = 256, c.per_thread = 32;
-    else if (vocab <= 16384) c.threads = 512, c.per_thread = 32;
-    else c.threads = 1024, c.per_thread = 32;
+    const int most = 1024 * 8 * vec;
+    c.segments = (int)(((size_t)vocab + most - 1) / most);
+    const size_t even = ((size_t)vocab + c.segments - 1) / c.segments, line = kLineBytes / 2;
+    c.length = (int)((even + line - 1) / line * line);  // stretches of an aligned row begin on lines
+    const int n = c.length < vocab ? c.length : vocab;
+    if (c.segments > 1) c.threads = 1024, c.iters = 8;
+    else if (n <= 512) c.threads = 64, c.iters = 8 / vec;
+    else if (n <= 2048) c.threads = 64, c.iters = 32 / vec;
+    else if (n <= 4096) c.threads = 256, c.iters = 16 / vec;
+    else if (n <= 8192) c.threads = 256, c.iters = 32 / vec;
+    else if (n <= 16384) c.threads = vec == 4 ? 1024 : 512, c.iters = 4;
+    else if (n <= 32768) c.threads = vec == 4 ? 1024 : 512, c.iters = 8;
+    else c.threads = 1024, c.iters = 8;
     return c;
+}
+
+// Calls launch(threads, iters), both as types with a ::value, for the shape that a row of one stretch takes.
+template <int V>
+struct Int {
+    static constexpr int value = V;
+};
+template <typename T, typename F>
+void for_shape(const RowCut& c, F&& launch) {
+    constexpr int vec = Elements<T>::kVec, wide = vec == 4 ? 1024 : 512;
+    if (c.threads == 64 && c.iters == 8 / vec) launch(Int<64>(), Int<8 / vec>());
+    else if (c.threads == 64) launch(Int<64>(), Int<32 / vec>());
+    else if (c.threads == 256 && c.iters == 16 / vec) launch(Int<256>(), Int<16 / vec>());
+    else if (c.threads == 256) launch(Int<256>(), Int<32 / vec>());
+    else if (c.threads == wide && c.iters == 4) launch(Int<wide>(), Int<4>());
+    else if (c.threads == wide) launch(Int<wide>(), Int<8>());
+    else launch(Int<1024>(), Int<8>());
 }
 
 }  // namespace mcc

@@ -9,6 +9,9 @@
 
 namespace mcc {
 
+constexpr int kLineBytes = 128;  // of the L2 cache
+__host__ __device__ inline bool whole_lines(const void* p) { return reinterpret_cast<uintptr_t>(p) % kLineBytes == 0; }
+
 // Element types of a tensor; everything computed from one is held in 32 bits and rounded once, to
 // nearest even, when it is stored.
 template <typename T>
@@ -29,33 +32,43 @@ struct Elements<__bf16> {
     typedef __bf16 Vec __attribute__((ext_vector_type(8), aligned(2)));
 };
 
-// The vectors of 16 bytes that one of `threads` threads holds of a row of n elements: vector j of
-// thread t covers the elements from (j * threads + t) * kVec.  A vector that would reach behind the
-// row's end is read from the row's last kVec elements instead, so that every load is unconditional
-// and in bounds; the elements it shares with the vector before it become `fill`, as do those of
-// vectors that lie behind the end altogether.  Rows shorter than a vector are read one by one.
-// 16-byte accesses need no more than the alignment of an element (unaligned access is enabled on
-// this platform), so row strides and base pointers are free.  Rows are streamed past the caches' replacement
-// order: every element is read once (32768 x 4096 bf16 backward: 156 -> 143 us; logits of 4096 x 32768 f32:
-// 94 -> 85 us).  A row that does not begin on a cache line is read through them, for its waves share the lines
-// where they meet (32768 x 4097 f32: 207 us, streamed 215 us).
-__host__ __device__ inline bool streamed(const void* row) { return (reinterpret_cast<uintptr_t>(row) & 127) == 0; }
+// The same number, which the compiler takes for a new one: indexes computed from it are computed where they are
+// needed instead of being held in registers since the loads.
+__device__ __forceinline__ int again(int t) {
+    asm volatile("" : "+v"(t));
+    return t;
+}
 
-template <typename T, int THREADS, int ITERS>
+// The vectors of 16 bytes that one of THREADS threads holds of a row of n elements: vector j of thread t
+// covers the elements from first(j, t) = (j * THREADS + t) * kVec - lead.  lead is 0, so that a row's sums are
+// taken in the same order wherever it lies, but for SHIFTED, where it moves the vectors back to the cache line
+// that the row begins in: a wave's accesses are then whole lines whatever the row's alignment (gradients of
+// 4096 x 32003 f32 logits: 196 us without).  A vector that reaches over an end of the row is read from the
+// nearest kVec elements inside it, so that every load is unconditional and in bounds; those of them that are
+// not its own, and all of a vector outside the row, become `fill`.  Rows shorter than a vector are read one
+// by one.  16-byte accesses need no more than the alignment of an element (unaligned access is enabled on this
+// platform).
+// Rows are streamed past the caches' replacement order, for every element is read once (32768 x 4096 bf16 norm,
+// backward: 156 -> 143 us; 4096 x 32768 f32 log probabilities: 94 -> 85 us).
+template <typename T, int THREADS, int ITERS, bool SHIFTED = false>
 struct RowVectors {
     static constexpr int kVec = Elements<T>::kVec;
     typedef typename Elements<T>::Vec Vec;
     Vec raw[ITERS];
+    int lead;
 
-    static __device__ __forceinline__ int first(int j, int t) { return (j * THREADS + t) * kVec; }
+    __device__ __forceinline__ int first(int j, int t) const { return (j * THREADS + t) * kVec - (SHIFTED ? lead : 0); }
     // where vector j of thread t is read from (rows of at least kVec elements)
-    static __device__ __forceinline__ int place(int j, int t, int n) {
-        const int e = first(j, t);
-        return e < n - kVec ? e : n - kVec;
+    __device__ __forceinline__ int place(int j, int t, int n) const {
+        const int e = first(j, t), f = SHIFTED && e < 0 ? 0 : e;
+        return f < n - kVec ? f : n - kVec;
     }
 
-    template <bool STREAM>
-    __device__ __forceinline__ void load_as(const T* row, int t, int n) {
+    // STREAM false: the row is read again soon.  `before`: elements from the line's start to the row's (SHIFTED;
+    // n + before at most what is held).
+    template <bool STREAM = true>
+    __device__ __forceinline__ void load(const T* row, int t, int n, int before = 0) {
+        lead = n >= kVec ? before : 0;
         if (n >= kVec) {
 #pragma unroll
             for (int j = 0; j < ITERS; ++j) {
@@ -66,52 +79,60 @@ struct RowVectors {
 #pragma unroll
             for (int j = 0; j < ITERS; ++j)
 #pragma unroll
-                for (int k = 0; k < kVec; ++k) raw[j][k] = first(j, t) + k < n ? row[first(j, t) + k] : (T)0.0f;
+                for (int k = 0; k < kVec; ++k) raw[j][k] = holds(j, k, t, n) ? row[index(j, k, t, n)] : (T)0.0f;
         }
     }
-    __device__ __forceinline__ void load(const T* row, int t, int n) {
-        if (streamed(row)) load_as<true>(row, t, n);
-        else load_as<false>(row, t, n);
+    // The same numbers, which the compiler takes for new ones: 16-bit numbers are then converted once more in the
+    // pass that follows instead of being held as 32 bits since the last.
+    __device__ __forceinline__ void convert_again() {
+        if (sizeof(T) == 4) return;
+        typedef uint32_t Words __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int j = 0; j < ITERS; ++j) {
+            Words w = __builtin_bit_cast(Words, raw[j]);
+            asm volatile("" : "+v"(w));
+            raw[j] = __builtin_bit_cast(Vec, w);
+        }
+    }
+    // whether vectors j of all threads lie inside the row (the same for every thread)
+    __device__ __forceinline__ bool whole(int j, int n) const {
+        return (j > 0 || !SHIFTED || lead == 0) && first(j + 1, 0) <= n;
     }
     __device__ __forceinline__ void fill_tail(int t, int n, T fill) {
 #pragma unroll
         for (int j = 0; j < ITERS; ++j) {
-            if ((j + 1) * THREADS * kVec <= n) continue;  // the same for every thread
-            const int e = first(j, t), at = n >= kVec ? place(j, t, n) : e;
+            if (whole(j, n)) continue;
+            const int u = again(t);
 #pragma unroll
             for (int k = 0; k < kVec; ++k)
-                if (at + k < e || at + k >= n) raw[j][k] = fill;
+                if (!holds(j, k, u, n)) raw[j][k] = fill;
         }
     }
-    // Index of element k of vector j in the row; not less than n, or less than first(), for one that
-    // fill_tail() filled.
-    static __device__ __forceinline__ int index(int j, int k, int t, int n) {
+    // Index of element k of vector j in the row, and whether it is the vector's own.
+    __device__ __forceinline__ int index(int j, int k, int t, int n) const {
         return (n >= kVec ? place(j, t, n) : first(j, t)) + k;
     }
-    static __device__ __forceinline__ bool holds(int j, int k, int t, int n) {
-        const int i = index(j, k, t, n);
-        return i >= first(j, t) && i < n;
+    __device__ __forceinline__ bool holds(int j, int k, int t, int n) const {
+        const int i = index(j, k, t, n), e = first(j, t);
+        return i >= e && i < n && (!SHIFTED || i - e < kVec);
+    }
+    // Stores numbers for vector j of thread t, past the caches as well: whole where the vector lies inside the
+    // row, else its own elements one by one.
+    __device__ __forceinline__ void store(T* row, int j, int t, int n, const float (&v)[kVec]) const {
+        const int e = first(j, t);
+        if ((!SHIFTED || e >= 0) && e + kVec <= n) {
+            Vec out;
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) out[k] = (T)v[k];
+            __builtin_nontemporal_store(out, reinterpret_cast<Vec*>(row + e));
+        } else if (e < n) {
+            const int u = again(t);
+#pragma unroll
+            for (int k = 0; k < kVec; ++k)
+                if (holds(j, k, u, n)) row[index(j, k, u, n)] = (T)v[k];
+        }
     }
 };
-
-// Stores vector j of thread t, past the caches as well: whole where it lies inside the row, else its elements one by one.
-template <typename T, int THREADS, int ITERS>
-__device__ __forceinline__ void store_row_vector(T* row, int j, int t, int n,
-                                                 const float (&v)[Elements<T>::kVec]) {
-    typedef RowVectors<T, THREADS, ITERS> Row;
-    typedef typename Row::Vec Vec;
-    const int e = Row::first(j, t);
-    if (e + Row::kVec <= n) {
-        Vec out;
-#pragma unroll
-        for (int k = 0; k < Row::kVec; ++k) out[k] = (T)v[k];
-        __builtin_nontemporal_store(out, reinterpret_cast<Vec*>(row + e));
-    } else if (e < n) {
-#pragma unroll
-        for (int k = 0; k < Row::kVec; ++k)
-            if (Row::holds(j, k, t, n)) row[Row::index(j, k, t, n)] = (T)v[k];
-    }
-}
 
 // ---- reductions: the same order on every call -------------------------------------------------
 struct Sum {

@@ -34,13 +34,6 @@ __device__ __forceinline__ float of_key(uint32_t k) {
 // A candidate: larger is likelier, and among equal logits the lower token is larger.
 __device__ __forceinline__ uint64_t candidate(float z, uint32_t id) { return (uint64_t)key_of(z) << 32 | (uint32_t)~id; }
 
-// The same number, which the compiler takes for a new one: indexes computed from it are computed where they are
-// needed instead of being held in registers since the loads.
-__device__ __forceinline__ int again(int t) {
-    asm volatile("" : "+v"(t));
-    return t;
-}
-
 template <int WAVES>
 struct TopScratch {
     static constexpr int kCandidates = WAVES == 1 ? 256 : 512;
@@ -103,11 +96,12 @@ __device__ __forceinline__ float lower_bound_of(float thread_max, int top, TopSc
 // fewer allowed tokens than `top` it is what the others were masked with.  Else the number is found by
 // bisection over the bits of its key.
 template <typename ROW, int WAVES, int ITERS>
-__device__ __forceinline__ void select_among_ties(const ROW& r, int n, uint32_t first_id, int top, float bound,
+__device__ __forceinline__ void select_among_ties(ROW& r, int n, uint32_t first_id, int top, float bound,
                                                   TopScratch<WAVES>& lds, int t, int wave, int lane) {
     int turn = 0;
     auto count = [&](auto test) {
         int c = 0;
+        r.convert_again();
 #pragma unroll
         for (int j = 0; j < ITERS; ++j) {
             const int u = again(t);
@@ -118,11 +112,12 @@ __device__ __forceinline__ void select_among_ties(const ROW& r, int n, uint32_t 
         turn ^= 1;
         return total_of<WAVES>(c, lds.totals, turn, wave, lane);
     };
-    auto number = [&](float z, int j, int k, int u) { return z >= -__builtin_inff() && ROW::holds(j, k, u, n); };
+    auto number = [&](float z, int j, int k, int u) { return z >= -__builtin_inff() && r.holds(j, k, u, n); };
     float f = 0.0f;
     const bool numbers = count(number) >= top;  // if not, all numbers are above and NaN are the ties
     if (numbers) {
         float least[1] = {__builtin_inff()};
+        r.convert_again();
 #pragma unroll
         for (int j = 0; j < ITERS; ++j)
 #pragma unroll
@@ -153,8 +148,9 @@ __device__ __forceinline__ void select_among_ties(const ROW& r, int n, uint32_t 
         }
     }
     auto above = [&](float z, int j, int k, int u) { return numbers ? z > f : number(z, j, k, u); };
-    auto equal = [&](float z, int j, int k, int u) { return (numbers ? z == f : !(z == z)) && ROW::holds(j, k, u, n); };
+    auto equal = [&](float z, int j, int k, int u) { return (numbers ? z == f : !(z == z)) && r.holds(j, k, u, n); };
     const int n_above = count(above);
+    r.convert_again();
     __syncthreads();
     if (t == 0) lds.count = 0;
     __syncthreads();
@@ -173,7 +169,7 @@ __device__ __forceinline__ void select_among_ties(const ROW& r, int n, uint32_t 
             lower += __builtin_popcountll(b & below);
             if (above(z, j, k, u)) {
                 const int at = atomicAdd(&lds.count, 1);
-                if (at < lds.kCandidates) lds.list[at] = candidate(z, first_id + ROW::index(j, k, u, n));
+                if (at < lds.kCandidates) lds.list[at] = candidate(z, first_id + r.index(j, k, u, n));
             }
         }
         turn ^= 1;
@@ -184,7 +180,7 @@ __device__ __forceinline__ void select_among_ties(const ROW& r, int n, uint32_t 
         for (int k = 0; k < ROW::kVec; ++k) {
             const float z = (float)r.raw[j][k];
             if (equal(z, j, k, u)) {
-                if (at < top) lds.list[at] = candidate(z, first_id + ROW::index(j, k, u, n));
+                if (at < top) lds.list[at] = candidate(z, first_id + r.index(j, k, u, n));
                 ++at;
             }
         }
@@ -197,12 +193,12 @@ __device__ __forceinline__ void select_among_ties(const ROW& r, int n, uint32_t 
 // The candidates of a stretch, unordered, in lds.list; returns their number (at least `top`, at most
 // kCandidates).  n >= top.
 template <typename ROW, int WAVES, int ITERS>
-__device__ __forceinline__ int find_candidates(const ROW& r, int n, uint32_t first_id, int top, float thread_max,
+__device__ __forceinline__ int find_candidates(ROW& r, int n, uint32_t first_id, int top, float thread_max,
                                                TopScratch<WAVES>& lds, int t, int wave, int lane) {
     const float bound = lower_bound_of<WAVES>(thread_max, top, lds, t, wave, lane);
     auto push = [&](float z, int j, int k) {
         const int at = atomicAdd(&lds.count, 1);
-        if (at < lds.kCandidates) lds.list[at] = candidate(z, first_id + ROW::index(j, k, again(t), n));
+        if (at < lds.kCandidates) lds.list[at] = candidate(z, first_id + r.index(j, k, again(t), n));
     };
     if (bound > -__builtin_inff()) {  // filled elements do not reach it
         if (thread_max >= bound) {
@@ -221,7 +217,7 @@ __device__ __forceinline__ int find_candidates(const ROW& r, int n, uint32_t fir
 #pragma unroll
             for (int k = 0; k < ROW::kVec; ++k) {
                 const float z = (float)r.raw[j][k];
-                if (z >= bound && ROW::holds(j, k, u, n)) push(z, j, k);
+                if (z >= bound && r.holds(j, k, u, n)) push(z, j, k);
             }
         }
     }
@@ -283,11 +279,11 @@ __device__ __forceinline__ bool token_of(const TokenLogProbs& a, size_t row, flo
 
 // One stretch a workgroup.  ONE: the row is one stretch, and the results are written; else `stats` and
 // `best` [rows * segments][top] are.
-template <typename T, int THREADS, int PER_THREAD, bool TOP, bool ONE>
+template <typename T, int THREADS, int ITERS, bool TOP, bool ONE>
 __global__ __launch_bounds__(THREADS, 8) void token_log_probs_kernel(TokenLogProbs a, int segments, int length,
                                                                   SoftmaxStats* stats, uint64_t* best) {
-    constexpr int kIters = PER_THREAD / Elements<T>::kVec, kWaves = THREADS / 64;
-    typedef RowVectors<T, THREADS, kIters> Row;
+    constexpr int kWaves = THREADS / 64;
+    typedef RowVectors<T, THREADS, ITERS> Row;
     __shared__ float slots[3 * kWaves];
     __shared__ TopScratch<TOP ? kWaves : 1> lds;
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
@@ -304,7 +300,7 @@ __global__ __launch_bounds__(THREADS, 8) void token_log_probs_kernel(TokenLogPro
     const bool has_token = ONE && t == 0 && token_of<T>(a, row, token_logit);
     r.fill_tail(t, n, (T)-__builtin_inff());
     float thread_max;
-    const SoftmaxStats st = stats_of<Row, kWaves, kIters>(r, a.log2_scale, slots, wave, lane, thread_max);
+    const SoftmaxStats st = stats_of<Row, kWaves, ITERS>(r, a.log2_scale, slots, wave, lane, thread_max);
     RowResult result{};
     if (ONE)
         result = finish_row(a, row, st, token_logit, has_token, t == 0);
@@ -312,7 +308,7 @@ __global__ __launch_bounds__(THREADS, 8) void token_log_probs_kernel(TokenLogPro
         stats[row * segments + segment] = st;
     if constexpr (TOP) {
         const int top = a.top < n ? a.top : n;
-        const int found = find_candidates<Row, kWaves, kIters>(r, n, (uint32_t)from, top, thread_max, lds, t, wave, lane);
+        const int found = find_candidates<Row, kWaves, ITERS>(r, n, (uint32_t)from, top, thread_max, lds, t, wave, lane);
         rank_candidates<THREADS>(lds.list, found, lds.rank, t);
         for (int i = t; i < found; i += THREADS) {
             const uint64_t mine = lds.list[i];
@@ -409,20 +405,26 @@ __global__ __launch_bounds__(kJoinThreads) void token_log_probs_join_kernel(Toke
 // ---- backward -----------------------------------------------------------------------------------
 // A stream of logits in and gradients out; the row's numbers are known beforehand.  grad_logits may be
 // logits (one thread owns an element).
-constexpr int kGradThreads = 256, kGradPerThread = 16;
+constexpr int kGradThreads = 256, kGradPerThread = 16, kGradLength = kGradThreads * kGradPerThread;
 template <typename T, bool ENTROPY>
 __global__ __launch_bounds__(kGradThreads) void token_log_probs_backward_kernel(
     const T* logits, size_t stride, const int32_t* tokens, const float* lse, const float* entropy,
     const float* grad_log_prob, const float* grad_entropy, T* grad_logits, size_t grad_stride, int segments, int vocab,
     float inv_temperature) {
-    constexpr int kIters = kGradPerThread / Elements<T>::kVec, kLength = kGradThreads * kGradPerThread;
-    typedef RowVectors<T, kGradThreads, kIters> Row;
+    constexpr int kIters = kGradPerThread / Elements<T>::kVec;
+    typedef RowVectors<T, kGradThreads, kIters, true> Row;
     const int t = threadIdx.x;
     const size_t row = blockIdx.x / (unsigned)segments;
-    const int from = (int)(blockIdx.x % (unsigned)segments) * kLength;
-    const int n = vocab - from < kLength ? vocab - from : kLength;
+    const int segment = (int)(blockIdx.x % (unsigned)segments);
+    // the row is cut at whole lines: the first stretch is shorter by what the row begins behind one
+    const T* begin = logits + row * stride;
+    const int behind = (int)((reinterpret_cast<uintptr_t>(begin) & (kLineBytes - 1)) / sizeof(T));
+    const int from = segment ? segment * kGradLength - behind : 0;
+    const int to = vocab - from < kGradLength - (segment ? 0 : behind) ? vocab : (segment + 1) * kGradLength - behind;
+    const int n = to - from;
+    if (n <= 0) return;
     Row r;
-    r.load(logits + row * stride + from, t, n);
+    r.load(begin + from, t, n, segment ? 0 : behind);
     const int32_t token = tokens ? tokens[row] : -1;
     const float l = lse[row], big_h = ENTROPY ? entropy[row] : 0.0f;
     const float g = grad_log_prob && token >= 0 && token < vocab ? grad_log_prob[row] : 0.0f;
@@ -443,13 +445,13 @@ __global__ __launch_bounds__(kGradThreads) void token_log_probs_backward_kernel(
         if (here) {
 #pragma unroll
             for (int k = 0; k < Row::kVec; ++k)
-                if (from + Row::index(j, k, t, n) == token) v[k] += gt;
+                if (from + r.index(j, k, t, n) == token) v[k] += gt;
         }
         if (zero) {
 #pragma unroll
             for (int k = 0; k < Row::kVec; ++k) v[k] = 0.0f;
         }
-        store_row_vector<T, kGradThreads, kIters>(grad_logits + row * grad_stride + from, j, t, n, v);
+        r.store(grad_logits + row * grad_stride + from, j, t, n, v);
     }
 }
 
@@ -458,30 +460,24 @@ size_t stats_nbytes(size_t rows, const RowCut& c) { return (rows * c.segments * 
 
 template <typename T, bool TOP>
 hipError_t launch_rows(hipStream_t stream, const TokenLogProbs& a, const RowCut& c) {
-#define MCC_ROWS(THREADS, PER_THREAD)                                                                           \
-    if (c.threads == THREADS && c.per_thread == PER_THREAD)                                                     \
-    hipLaunchKernelGGL((token_log_probs_kernel<T, THREADS, PER_THREAD, TOP, true>), dim3((unsigned)a.rows),     \
-                       dim3(THREADS), 0, stream, a, 1, c.length, (SoftmaxStats*)nullptr, (uint64_t*)nullptr)
-    MCC_ROWS(64, 8);
-    MCC_ROWS(64, 32);
-    MCC_ROWS(256, 16);
-    MCC_ROWS(256, 32);
-    MCC_ROWS(512, 32);
-    MCC_ROWS(1024, 32);
-#undef MCC_ROWS
+    for_shape<T>(c, [&](auto threads, auto iters) {
+        constexpr int THREADS = decltype(threads)::value, ITERS = decltype(iters)::value;
+        hipLaunchKernelGGL((token_log_probs_kernel<T, THREADS, ITERS, TOP, true>), dim3((unsigned)a.rows), dim3(THREADS), 0,
+                           stream, a, 1, c.length, (SoftmaxStats*)nullptr, (uint64_t*)nullptr);
+    });
     return hipGetLastError();
 }
 
 template <typename T, bool TOP>
 hipError_t launch_stretches(hipStream_t stream, const TokenLogProbs& a, const RowCut& c, SoftmaxStats* stats, uint64_t* best) {
-    hipLaunchKernelGGL((token_log_probs_kernel<T, 1024, 32, TOP, false>), dim3((unsigned)(a.rows * c.segments)), dim3(1024),
+    hipLaunchKernelGGL((token_log_probs_kernel<T, 1024, 8, TOP, false>), dim3((unsigned)(a.rows * c.segments)), dim3(1024),
                        0, stream, a, c.segments, c.length, stats, best);
     return hipGetLastError();
 }
 
 template <typename T>
 hipError_t forward(hipStream_t stream, const TokenLogProbs& a, void* workspace) {
-    const RowCut c = cut_rows(a.vocab);
+    const RowCut c = cut_rows(a.vocab, Elements<T>::kVec);
     const bool top = a.top > 0 && (a.top_ids || a.top_log_probs);
     if (c.segments == 1) return top ? launch_rows<T, true>(stream, a, c) : launch_rows<T, false>(stream, a, c);
     SoftmaxStats* stats = static_cast<SoftmaxStats*>(workspace);
@@ -498,8 +494,10 @@ template <typename T>
 hipError_t backward(hipStream_t stream, const void* logits, size_t stride, const int32_t* tokens, const float* lse,
                     const float* entropy, const float* grad_log_prob, const float* grad_entropy, void* grad_logits,
                     size_t grad_stride, size_t rows, int vocab, float inv_temperature) {
-    constexpr int length = kGradThreads * kGradPerThread;
-    const int segments = (int)(((size_t)vocab + length - 1) / length);
+    // one more line for rows that do not begin on one
+    const bool aligned = whole_lines(logits) && (rows == 1 || stride * sizeof(T) % kLineBytes == 0);
+    const size_t reach = (size_t)vocab + (aligned ? 0 : kLineBytes / sizeof(T) - 1);
+    const int segments = (int)((reach + kGradLength - 1) / kGradLength);
     const dim3 grid((unsigned)(rows * segments)), block(kGradThreads);
     if (grad_entropy)
         hipLaunchKernelGGL((token_log_probs_backward_kernel<T, true>), grid, block, 0, stream, static_cast<const T*>(logits),
@@ -514,8 +512,8 @@ hipError_t backward(hipStream_t stream, const void* logits, size_t stride, const
 
 }  // namespace
 
-size_t token_log_probs_workspace_nbytes(size_t rows, int vocab, int top) {
-    const RowCut c = cut_rows(vocab);
+size_t token_log_probs_workspace_nbytes(ElementType type, size_t rows, int vocab, int top) {
+    const RowCut c = cut_rows(vocab, type == ElementType::F32 ? 4 : 8);
     if (c.segments == 1) return 0;
     return stats_nbytes(rows, c) + rows * c.segments * (size_t)top * sizeof(uint64_t);
 }
