@@ -947,16 +947,11 @@ struct RowsCheck {
         if (!std::isfinite(t) || !(t > 0.0f) || !std::isfinite(2.0f / t)) return say("requires a positive finite temperature");
         return true;
     }
-    // workgroups of one launch
-    bool groups(size_t per_row) const {
-        return rows <= kIntMax / per_row || say("rows times row length exceed what one call takes");
-    }
 };
 
 float log2_scale(float temperature) { return (float)(1.44269504088896340736 / (double)temperature); }
 
-// No kernel cuts rows into stretches shorter than 4096 elements.
-size_t most_stretches(size_t cols) { return (cols + 4095) / 4096 + 1; }
+static_assert(mcc::kMostTop == MCC_MOST_TOP, "the kernels' scratch holds the most alternatives");
 
 }  // namespace
 
@@ -1013,7 +1008,7 @@ int mcc_layer_norm_backward(void* stream, const void* grad_out, size_t grad_out_
 
 size_t mcc_token_log_probs_workspace_nbytes(size_t rows, size_t vocab, size_t top, int element) {
     RowsCheck c{"token_log_probs", rows, vocab};
-    if (!c.shape(element) || top > MCC_MOST_TOP || top > vocab || !c.groups(most_stretches(vocab))) return 0;
+    if (!c.shape(element) || top > MCC_MOST_TOP || top > vocab) return 0;
     return mcc::token_log_probs_workspace_nbytes(c.type, rows, (int)vocab, (int)top);
 }
 
@@ -1026,7 +1021,7 @@ int mcc_token_log_probs(void* stream, const void* logits, size_t logits_nbytes, 
     if (!c.shape(element) || !c.temperature(temperature)) return MCC_E_INVALID;
     if (top > MCC_MOST_TOP || top > vocab)
         return fail(MCC_E_INVALID, "token_log_probs gives at most 128 and at most vocab alternatives");
-    if (!c.tensor("logits", {logits, logits_nbytes, logits_stride}) || !c.groups(most_stretches(vocab)) ||
+    if (!c.tensor("logits", {logits, logits_nbytes, logits_stride}) ||
         !c.numbers("tokens", tokens, tokens_nbytes, rows, true) ||
         !c.numbers("log_prob", log_prob, log_prob_nbytes, rows, true) ||
         !c.numbers("entropy", entropy, entropy_nbytes, rows, true) || !c.numbers("lse", lse, lse_nbytes, rows, true) ||
@@ -1050,7 +1045,7 @@ int mcc_token_log_probs_backward(void* stream, const void* logits, size_t logits
                                  size_t vocab, int element, float temperature) {
     RowsCheck c{"token_log_probs_backward", rows, vocab};
     const RowsArg la{logits, logits_nbytes, logits_stride}, ga{grad_logits, grad_logits_nbytes, grad_logits_stride};
-    if (!c.shape(element) || !c.temperature(temperature) || !c.groups(most_stretches(vocab)) || !c.tensor("logits", la) ||
+    if (!c.shape(element) || !c.temperature(temperature) || !c.tensor("logits", la) ||
         !c.tensor("grad_logits", ga) || !c.apart("grad_logits", ga, "logits", la) ||
         !c.numbers("tokens", tokens, tokens_nbytes, rows, !grad_log_prob) || !c.numbers("lse", lse, lse_nbytes, rows, false) ||
         !c.numbers("entropy", entropy, entropy_nbytes, rows, !grad_entropy) ||

@@ -117,8 +117,12 @@ __device__ __forceinline__ void write_stretch(const GradientScale& c, T* out, in
         r.store(out, j, t, n, v);
     }
 }
-// The elements that the teacher's entries name, by the first wave; a barrier lies between the writes of the
-// row and this.
+// All waves' gradient is in memory, past the point where a second store to an element could overtake the first.
+__device__ __forceinline__ void gradient_written() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+// The elements that the teacher's entries name, by the first wave, after gradient_written().
 template <typename T>
 __device__ __forceinline__ void patch_entries(const DistillTop& a, const GradientScale& c, T* out,
                                               const EntryScratch& lds, int t) {
@@ -165,7 +169,7 @@ __global__ __launch_bounds__(THREADS, 8) void distill_row_kernel(DistillTop a) {
     const GradientScale c(a, row, st.m, st.s, lds.sum);
     T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
     write_stretch<T, THREADS, ITERS>(c, out, n, r, t);
-    __syncthreads();
+    gradient_written();
     patch_entries(a, c, out, lds, t);
 }
 
@@ -248,12 +252,23 @@ hipError_t distill(hipStream_t stream, const DistillTop& a) {
 }  // namespace
 
 hipError_t launch_distill_top(hipStream_t stream, ElementType type, const DistillTop& a) {
-    switch (type) {
-        case ElementType::F32: return distill<float>(stream, a);
-        case ElementType::F16: return distill<_Float16>(stream, a);
-        case ElementType::BF16: return distill<__bf16>(stream, a);
+    hipError_t e = hipSuccess;
+    for (size_t done = 0; done < a.rows && e == hipSuccess; done += kMostLaunchRows) {
+        DistillTop p = a;
+        p.rows = a.rows - done < kMostLaunchRows ? a.rows - done : kMostLaunchRows;
+        p.logits = static_cast<const char*>(a.logits) + done * a.stride * element_size(type);
+        p.ids = a.ids + done * a.top;
+        p.teacher = a.teacher + done * a.top;
+        if (a.weight) p.weight = a.weight + done;
+        if (a.loss) p.loss = a.loss + done;
+        if (a.grad) p.grad = static_cast<char*>(a.grad) + done * a.grad_stride * element_size(type);
+        switch (type) {
+            case ElementType::F32: e = distill<float>(stream, p); break;
+            case ElementType::F16: e = distill<_Float16>(stream, p); break;
+            case ElementType::BF16: e = distill<__bf16>(stream, p); break;
+        }
     }
-    return hipErrorInvalidValue;
+    return e;
 }
 
 }  // namespace mcc

@@ -152,6 +152,10 @@ hipError_t launch_adam_update(hipStream_t stream, float* param, const float* gra
 // ---- row-wise operators --------------------------------------------------------------------------
 // Strides are elements between the starts of two rows; rows and lengths are at least 1.
 enum class ElementType { F32, F16, BF16 };
+constexpr size_t element_size(ElementType type) { return type == ElementType::F32 ? 4 : 2; }
+// Rows of one launch of a grid that grows with them: at 1024 threads a row, half of the 2^32 threads that a
+// launch may have.  More rows go out as several launches.
+constexpr size_t kMostLaunchRows = (size_t)1 << 21;
 
 // y = (x - mean) * rstd * gain + bias (layer_norm.hip); gain, bias, mean and rstd may be null, y may
 // be x with the same stride.

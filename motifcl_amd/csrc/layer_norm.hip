@@ -414,9 +414,12 @@ hipError_t backward(hipStream_t stream, const void* dv, size_t d_stride, const v
             hipLaunchKernelGGL(layer_norm_columns_long_kernel<T>,
                                dim3((unsigned)((n + kLongThreads - 1) / kLongThreads), (unsigned)groups),
                                dim3(kLongThreads), 0, stream, d, d_stride, x, x_stride, mean, rstd, pg, pb, stride, rows, n);
-        if (gx)
-            hipLaunchKernelGGL(layer_norm_grad_x_long_kernel<T>, dim3((unsigned)rows), dim3(kLongThreads), 0, stream, d,
-                               d_stride, x, x_stride, mean, rstd, gain, gx, g_stride, n, inv_n);
+        for (size_t done = 0; gx && done < rows; done += kMostLaunchRows) {
+            const size_t part = rows - done < kMostLaunchRows ? rows - done : kMostLaunchRows;
+            hipLaunchKernelGGL(layer_norm_grad_x_long_kernel<T>, dim3((unsigned)part), dim3(kLongThreads), 0, stream,
+                               d + done * d_stride, d_stride, x + done * x_stride, x_stride, mean + done, rstd + done, gain,
+                               gx + done * g_stride, g_stride, n, inv_n);
+        }
     }
 #undef MCC_NORM_BACKWARD
     const hipError_t e = hipGetLastError();
@@ -431,12 +434,19 @@ hipError_t backward(hipStream_t stream, const void* dv, size_t d_stride, const v
 hipError_t launch_layer_norm(hipStream_t stream, ElementType type, const void* x, size_t x_stride, const float* gain,
                              const float* bias, void* y, size_t y_stride, float* mean, float* rstd, size_t rows, int n,
                              float eps) {
-    switch (type) {
-        case ElementType::F32: return forward<float>(stream, x, x_stride, gain, bias, y, y_stride, mean, rstd, rows, n, eps);
-        case ElementType::F16: return forward<_Float16>(stream, x, x_stride, gain, bias, y, y_stride, mean, rstd, rows, n, eps);
-        case ElementType::BF16: return forward<__bf16>(stream, x, x_stride, gain, bias, y, y_stride, mean, rstd, rows, n, eps);
+    hipError_t e = hipSuccess;
+    for (size_t done = 0; done < rows && e == hipSuccess; done += kMostLaunchRows) {
+        const size_t part = rows - done < kMostLaunchRows ? rows - done : kMostLaunchRows;
+        const void* xp = static_cast<const char*>(x) + done * x_stride * element_size(type);
+        void* yp = static_cast<char*>(y) + done * y_stride * element_size(type);
+        float *m = mean ? mean + done : nullptr, *r = rstd ? rstd + done : nullptr;
+        switch (type) {
+            case ElementType::F32: e = forward<float>(stream, xp, x_stride, gain, bias, yp, y_stride, m, r, part, n, eps); break;
+            case ElementType::F16: e = forward<_Float16>(stream, xp, x_stride, gain, bias, yp, y_stride, m, r, part, n, eps); break;
+            case ElementType::BF16: e = forward<__bf16>(stream, xp, x_stride, gain, bias, yp, y_stride, m, r, part, n, eps); break;
+        }
     }
-    return hipErrorInvalidValue;
+    return e;
 }
 
 size_t layer_norm_backward_workspace_nbytes(ElementType type, size_t rows, int n) {

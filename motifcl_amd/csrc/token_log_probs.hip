@@ -455,11 +455,17 @@ __global__ __launch_bounds__(kGradThreads) void token_log_probs_backward_kernel(
     }
 }
 
+// Rows of one launch with `segments` workgroups a row.
+size_t launch_rows(int segments) {
+    const size_t rows = kMostLaunchRows / (size_t)segments;
+    return rows > 0 ? rows : 1;
+}
+
 // Workspace of a row cut into stretches: their statistics, then their entries.
 size_t stats_nbytes(size_t rows, const RowCut& c) { return (rows * c.segments * sizeof(SoftmaxStats) + 15) / 16 * 16; }
 
 template <typename T, bool TOP>
-hipError_t launch_rows(hipStream_t stream, const TokenLogProbs& a, const RowCut& c) {
+hipError_t launch_whole(hipStream_t stream, const TokenLogProbs& a, const RowCut& c) {
     for_shape<T>(c, [&](auto threads, auto iters) {
         constexpr int THREADS = decltype(threads)::value, ITERS = decltype(iters)::value;
         hipLaunchKernelGGL((token_log_probs_kernel<T, THREADS, ITERS, TOP, true>), dim3((unsigned)a.rows), dim3(THREADS), 0,
@@ -479,7 +485,7 @@ template <typename T>
 hipError_t forward(hipStream_t stream, const TokenLogProbs& a, void* workspace) {
     const RowCut c = cut_rows(a.vocab, Elements<T>::kVec);
     const bool top = a.top > 0 && (a.top_ids || a.top_log_probs);
-    if (c.segments == 1) return top ? launch_rows<T, true>(stream, a, c) : launch_rows<T, false>(stream, a, c);
+    if (c.segments == 1) return top ? launch_whole<T, true>(stream, a, c) : launch_whole<T, false>(stream, a, c);
     SoftmaxStats* stats = static_cast<SoftmaxStats*>(workspace);
     uint64_t* best = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + stats_nbytes(a.rows, c));
     const hipError_t e = top ? launch_stretches<T, true>(stream, a, c, stats, best)
@@ -515,34 +521,59 @@ hipError_t backward(hipStream_t stream, const void* logits, size_t stride, const
 size_t token_log_probs_workspace_nbytes(ElementType type, size_t rows, int vocab, int top) {
     const RowCut c = cut_rows(vocab, type == ElementType::F32 ? 4 : 8);
     if (c.segments == 1) return 0;
-    return stats_nbytes(rows, c) + rows * c.segments * (size_t)top * sizeof(uint64_t);
+    const size_t part = launch_rows(c.segments) < rows ? launch_rows(c.segments) : rows;  // reused by the next
+    return stats_nbytes(part, c) + part * c.segments * (size_t)top * sizeof(uint64_t);
 }
 
 hipError_t launch_token_log_probs(hipStream_t stream, ElementType type, const TokenLogProbs& a, void* workspace) {
-    switch (type) {
-        case ElementType::F32: return forward<float>(stream, a, workspace);
-        case ElementType::F16: return forward<_Float16>(stream, a, workspace);
-        case ElementType::BF16: return forward<__bf16>(stream, a, workspace);
+    const size_t most = launch_rows(cut_rows(a.vocab, type == ElementType::F32 ? 4 : 8).segments);
+    hipError_t e = hipSuccess;
+    for (size_t done = 0; done < a.rows && e == hipSuccess; done += most) {
+        TokenLogProbs p = a;
+        p.rows = a.rows - done < most ? a.rows - done : most;
+        p.logits = static_cast<const char*>(a.logits) + done * a.stride * element_size(type);
+        if (a.tokens) p.tokens = a.tokens + done;
+        if (a.log_prob) p.log_prob = a.log_prob + done;
+        if (a.entropy) p.entropy = a.entropy + done;
+        if (a.lse) p.lse = a.lse + done;
+        if (a.top_ids) p.top_ids = a.top_ids + done * a.top;
+        if (a.top_log_probs) p.top_log_probs = a.top_log_probs + done * a.top;
+        switch (type) {
+            case ElementType::F32: e = forward<float>(stream, p, workspace); break;
+            case ElementType::F16: e = forward<_Float16>(stream, p, workspace); break;
+            case ElementType::BF16: e = forward<__bf16>(stream, p, workspace); break;
+        }
     }
-    return hipErrorInvalidValue;
+    return e;
 }
 
 hipError_t launch_token_log_probs_backward(hipStream_t stream, ElementType type, const void* logits, size_t stride,
                                            const int32_t* tokens, const float* lse, const float* entropy,
                                            const float* grad_log_prob, const float* grad_entropy, void* grad_logits,
                                            size_t grad_stride, size_t rows, int vocab, float inv_temperature) {
-    switch (type) {
-        case ElementType::F32:
-            return backward<float>(stream, logits, stride, tokens, lse, entropy, grad_log_prob, grad_entropy, grad_logits,
-                                   grad_stride, rows, vocab, inv_temperature);
-        case ElementType::F16:
-            return backward<_Float16>(stream, logits, stride, tokens, lse, entropy, grad_log_prob, grad_entropy, grad_logits,
-                                      grad_stride, rows, vocab, inv_temperature);
-        case ElementType::BF16:
-            return backward<__bf16>(stream, logits, stride, tokens, lse, entropy, grad_log_prob, grad_entropy, grad_logits,
-                                    grad_stride, rows, vocab, inv_temperature);
+    const size_t most = launch_rows(vocab / kGradLength + 2), size = element_size(type);
+    hipError_t e = hipSuccess;
+    for (size_t done = 0; done < rows && e == hipSuccess; done += most) {
+        const size_t part = rows - done < most ? rows - done : most;
+        const void* z = static_cast<const char*>(logits) + done * stride * size;
+        void* g = static_cast<char*>(grad_logits) + done * grad_stride * size;
+        auto at = [&](auto* p) { return p ? p + done : nullptr; };
+        switch (type) {
+            case ElementType::F32:
+                e = backward<float>(stream, z, stride, at(tokens), at(lse), at(entropy), at(grad_log_prob), at(grad_entropy), g,
+                                    grad_stride, part, vocab, inv_temperature);
+                break;
+            case ElementType::F16:
+                e = backward<_Float16>(stream, z, stride, at(tokens), at(lse), at(entropy), at(grad_log_prob),
+                                       at(grad_entropy), g, grad_stride, part, vocab, inv_temperature);
+                break;
+            case ElementType::BF16:
+                e = backward<__bf16>(stream, z, stride, at(tokens), at(lse), at(entropy), at(grad_log_prob),
+                                     at(grad_entropy), g, grad_stride, part, vocab, inv_temperature);
+                break;
+        }
     }
-    return hipErrorInvalidValue;
+    return e;
 }
 
 }  // namespace mcc

@@ -491,6 +491,30 @@ def test_rows_beyond_32_bit_offsets(ops):
     assert torch.equal(out[-600:], want_dx)
 
 
+@pytest.mark.parametrize("rows, n", [((1 << 21) + 5, 3), ((1 << 20) + 3, 8200)])
+def test_more_rows_than_a_launch_takes(ops, rows, n):
+    # 2^21 workgroups a launch: one a row, or, in the gradient of the log probabilities, one a stretch of 4096
+    g = generator(n)
+    z = torch.empty(rows, n, dtype=torch.bfloat16, device="cuda")
+    z.normal_(generator=g)
+    tokens = torch.randint(0, n, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    ids = torch.randint(0, n, (rows, 2), generator=g, device="cuda", dtype=torch.int32)
+    teacher = torch.randn(rows, 2, generator=g, device="cuda")
+    r = ops.token_log_probs(z, tokens, top=2)
+    loss, dz = ops.distill_top(z, ids, teacher)
+    grad = ops.token_log_probs_backward(z, tokens, r.lse, r.entropy, r.entropy)
+    y, mean, rstd = ops.layer_norm(z)
+    for at in (slice(0, 5000), slice(rows // 2 - 2500, rows // 2 + 2500), slice(rows - 5000, rows)):
+        part = ops.token_log_probs(z[at], tokens[at], top=2)
+        for a, b in zip(r, part):
+            assert torch.equal(a[at], b)
+        part = ops.distill_top(z[at], ids[at], teacher[at])
+        assert torch.equal(loss[at], part[0]) and torch.equal(dz[at], part[1])
+        assert torch.equal(grad[at], ops.token_log_probs_backward(z[at], tokens[at], r.lse[at], r.entropy[at], r.entropy[at]))
+        part = ops.layer_norm(z[at])
+        assert torch.equal(y[at], part[0]) and torch.equal(mean[at], part[1]) and torch.equal(rstd[at], part[2])
+
+
 def run_all(ops, z, x, gain, tokens, ids, teacher):
     y, mean, rstd = ops.layer_norm(x, gain, None)
     dx, dgain, dbias = ops.layer_norm_backward(y, x, mean, rstd, gain)

@@ -83,7 +83,6 @@ def log_probs(L, z=P, zn=4 * 400, zs=100, tok=2 * P, tokn=16, lp=3 * P, lpn=16, 
     (dict(vocab=40000, zs=40000, zn=4 * 160000), "null"),
     (dict(vocab=40000, zs=40000, zn=4 * 160000, ws=P + 4, wsn=BIG), "16-byte"),
     (dict(vocab=40000, zs=40000, zn=4 * 160000, ws=P, wsn=100), "workspace is too small"),
-    (dict(rows=1 << 30, vocab=1 << 20, zs=1 << 20, zn=1 << 63), "what one call takes"),
 ])
 def test_token_log_probs_refuses(L, kwargs, needle):
     refused(L, log_probs(L, **kwargs), needle)
