@@ -258,13 +258,17 @@ def _out_rows(out, like, buf):
 
 
 def _numbers(t, dtype, shape, like, name):
-    """(pointer, bytes) of a contiguous tensor on the device of `like`; None gives a null pointer."""
+    """(pointer, bytes) of a contiguous tensor of 4-byte numbers on the device of `like`; None gives a null pointer."""
     if t is None:
         return None, 0
     if t.shape != shape or t.device != like.device:
         raise ValueError("%s: expected shape %s on %s, got %s on %s" % (name, tuple(shape), like.device, tuple(t.shape),
                                                                        t.device))
-    return _buf(t, dtype)
+    if t.dtype != dtype:
+        raise ValueError("expected dtype %s, got %s" % (dtype, t.dtype))
+    if not t.is_contiguous():
+        raise ValueError("expected a contiguous tensor")
+    return t.data_ptr(), 4 * t.numel()
 
 
 def _new(like, shape, dtype=torch.float32):
@@ -326,7 +330,7 @@ def layer_norm_backward(grad_out, x, mean, rstd, gain=None, bias=True, input_gra
     buf, rows, cols, element = _rows(x, "x")
     grad_buf = _same_rows(grad_out, x, "grad_out")
     grad_x, x_out = _out_rows(out, x, buf) if input_grad else (None, (None, 0, 0))
-    grad_gain = _new(x, cols) if gain is not None else None
+    grad_gain = torch.empty_like(gain) if gain is not None else None
     grad_bias = _new(x, cols) if bias else None
     shape, n = x.shape[:-1], 4 * cols
     need = 0 if grad_gain is None and grad_bias is None else L.mcc_layer_norm_backward_workspace_nbytes(rows, cols, element)
