@@ -357,8 +357,8 @@ hipError_t forward(hipStream_t stream, const void* xv, size_t x_stride, const fl
         if (rows < kManyRows) MCC_NORM_AS(THREADS, ITERS, SLOTS, 1);                   \
         else MCC_NORM_AS(THREADS, ITERS, SLOTS, ROWS);                                 \
     } while (0)
-    // Sixteen-bit rows are read with half the bytes of gain and bias to theirs that 32-bit rows need twice: sharing
-    // them pays there (16384 x 4096 bf16: 58 us alone, 53 us by two, 52 us by four; 8191 wide 145 us alone, 112 us by
+    // Gain and bias are 8 bytes an element from the caches, twice what a 16-bit row reads and writes: sharing them
+    // pays there (16384 x 4096 bf16: 58 us alone, 53 us by two rows, 52 us by four; 8191 wide 145 us alone, 112 us by
     // two), and not for f32 (32768 x 4096: 178 us alone, 188 us by two).
     constexpr int kRows = vec == 8 ? 4 : 1, kRows4 = vec == 8 ? 2 : 1;
     // a row is a wave's up to 32 elements a thread, then a workgroup's of 256, then of 1024 threads

@@ -2,8 +2,9 @@
 // With d = (z - max) k and k = log2(e) / temperature over the stretch:
 //     m = max z,  s = sum 2^d,  u = sum 2^d d
 // from which log sum e^(z / temperature) = m / temperature + log s and the entropy is log s - log(2) u / s.
-// Stretches are joined by m = max m_i, r_i = 2^((m_i - m) k), s = sum r_i s_i, u = sum r_i (u_i + s_i (m_i - m) k).  A stretch of -inf alone has m = -inf, s = u = 0; a NaN or
-// +inf makes s (and with it everything taken from the row) NaN.
+// Stretches are joined by m = max m_i, r_i = 2^((m_i - m) k), s = sum r_i s_i, u = sum r_i (u_i + s_i (m_i - m) k).
+// A stretch of -inf alone has m = -inf, s = u = 0; a NaN or +inf makes s (and with it everything taken from the
+// row) NaN.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -80,7 +81,8 @@ inline RowCut cut_rows(int vocab, int vec) {
     const int most = 1024 * 8 * vec;
     c.segments = (int)(((size_t)vocab + most - 1) / most);
     const size_t even = ((size_t)vocab + c.segments - 1) / c.segments, line = kLineBytes / 2;
-    c.length = (int)((even + line - 1) / line * line);  // stretches of an aligned row begin on lines
+    // stretches of an aligned row begin on lines; at most `most`, so that none is left empty
+    c.length = (int)((even + line - 1) / line * line);
     const int n = c.length < vocab ? c.length : vocab;
     if (c.segments > 1) c.threads = 1024, c.iters = 8;
     else if (n <= 512) c.threads = 64, c.iters = 8 / vec;

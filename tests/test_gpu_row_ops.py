@@ -491,6 +491,23 @@ def test_rows_beyond_32_bit_offsets(ops):
     assert torch.equal(out[-600:], want_dx)
 
 
+@pytest.mark.parametrize("vocab, dtype", [(8650753, torch.float32), (9000001, torch.float32), (35000003, torch.bfloat16)])
+def test_rows_of_very_many_stretches(ops, vocab, dtype):
+    # hundreds of stretches a row: every one holds something, and their entries are more than are ranked at once
+    z = logits_of(generator(vocab), 2, vocab, dtype)
+    tokens = torch.tensor([vocab - 1, 0], dtype=torch.int32, device="cuda")
+    check_log_probs(ops, z, tokens, 100, 1.0)
+    ids = torch.tensor([[vocab - 1, 0, 7]] * 2, dtype=torch.int32, device="cuda")
+    teacher = torch.tensor([[1.0, 0.5, 0.0]] * 2, device="cuda")
+    loss, grad = ops.distill_top(z, ids, teacher)
+    want_loss, want, _, p = rows64.distill_top(z, ids, teacher, None, 1.0)
+    wide = float(z.double().abs().max())
+    rows64.close(loss, want_loss, 400.0 + 16 * wide + 16 * math.log(vocab), 1, "loss")
+    scale = (140.0 + 8 * wide) * p
+    scale[:, [0, 7, vocab - 1]] += 140.0
+    rows64.close(grad, want, scale, 1, "grad")
+
+
 @pytest.mark.parametrize("rows, n", [((1 << 21) + 5, 3), ((1 << 20) + 3, 8200)])
 def test_more_rows_than_a_launch_takes(ops, rows, n):
     # 2^21 workgroups a launch: one a row, or, in the gradient of the log probabilities, one a stretch of 4096
