@@ -74,8 +74,9 @@ struct RowCut {
 // further, so that more CUs read them, does not pay for the launch that joins the stretches: one row of 32768
 // f32 takes 30.7 us from call to end whole and 34.6 us in eight stretches, 200 rows 35 and 39 us.
 // Sixteen-bit rows are bound by the vector units and want few waves, which share the work that is done once a
-// wave (distillation of 4096 x 16384 bf16: 56 us with 512 threads, 72 us with 1024); f32 rows are bound by
-// memory and want many (114 and 103 us).
+// wave: 64 numbers a thread (distillation of 16384 x 3001 bf16: 55 us in one wave, 67 us in four; of 4096 x 16384:
+// 56 us with 256 or 512 threads, 72 us with 1024).  f32 rows are bound by memory and want many (of 16384 x 3001 f32:
+// 83 us in two waves, 77 us in four; of 4096 x 16384: 114 us with 512 threads, 103 us with 1024).
 inline RowCut cut_rows(int vocab, int vec) {
     RowCut c;
     const int most = 1024 * 8 * vec;
@@ -87,11 +88,10 @@ inline RowCut cut_rows(int vocab, int vec) {
     if (c.segments > 1) c.threads = 1024, c.iters = 8;
     else if (n <= 512) c.threads = 64, c.iters = 8 / vec;
     else if (n <= 2048) c.threads = 64, c.iters = 32 / vec;
-    else if (n <= 4096) c.threads = 256, c.iters = 16 / vec;
-    else if (n <= 8192) c.threads = 256, c.iters = 32 / vec;
-    else if (n <= 16384) c.threads = vec == 4 ? 1024 : 512, c.iters = 4;
-    else if (n <= 32768) c.threads = vec == 4 ? 1024 : 512, c.iters = 8;
-    else c.threads = 1024, c.iters = 8;
+    else if (vec == 8) c.threads = n <= 4096 ? 64 : n <= 8192 ? 128 : n <= 16384 ? 256 : n <= 32768 ? 512 : 1024, c.iters = 8;
+    else if (n <= 4096) c.threads = 256, c.iters = 4;
+    else if (n <= 8192) c.threads = 256, c.iters = 8;
+    else c.threads = 1024, c.iters = n <= 16384 ? 4 : 8;
     return c;
 }
 
@@ -102,14 +102,21 @@ struct Int {
 };
 template <typename T, typename F>
 void for_shape(const RowCut& c, F&& launch) {
-    constexpr int vec = Elements<T>::kVec, wide = vec == 4 ? 1024 : 512;
+    constexpr int vec = Elements<T>::kVec;
     if (c.threads == 64 && c.iters == 8 / vec) launch(Int<64>(), Int<8 / vec>());
-    else if (c.threads == 64) launch(Int<64>(), Int<32 / vec>());
-    else if (c.threads == 256 && c.iters == 16 / vec) launch(Int<256>(), Int<16 / vec>());
-    else if (c.threads == 256) launch(Int<256>(), Int<32 / vec>());
-    else if (c.threads == wide && c.iters == 4) launch(Int<wide>(), Int<4>());
-    else if (c.threads == wide) launch(Int<wide>(), Int<8>());
-    else launch(Int<1024>(), Int<8>());
+    else if (c.threads == 64 && c.iters == 32 / vec) launch(Int<64>(), Int<32 / vec>());
+    else if constexpr (vec == 8) {
+        if (c.threads == 64) launch(Int<64>(), Int<8>());
+        else if (c.threads == 128) launch(Int<128>(), Int<8>());
+        else if (c.threads == 256) launch(Int<256>(), Int<8>());
+        else if (c.threads == 512) launch(Int<512>(), Int<8>());
+        else launch(Int<1024>(), Int<8>());
+    } else {
+        if (c.threads == 256 && c.iters == 4) launch(Int<256>(), Int<4>());
+        else if (c.threads == 256) launch(Int<256>(), Int<8>());
+        else if (c.iters == 4) launch(Int<1024>(), Int<4>());
+        else launch(Int<1024>(), Int<8>());
+    }
 }
 
 }  // namespace mcc
