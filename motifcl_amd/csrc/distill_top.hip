@@ -5,7 +5,8 @@
 // read once and the gradient is written once where the workgroup's registers hold the row; a longer row is read a
 // second time, as far as the registers and caches do not hold it.  The teacher's entries change `top` elements of a
 // row: the gradient is written without them first and those elements are written again behind a barrier, each by
-// the first of the entries that name it.
+// the first of the entries that name it.  Measured: 4096 x 32768 f32 190 us = 5.7 TB/s; 2048 x 128011 f32 493 us, of
+// whose 2.9 GB 0.8 are the second read.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -173,7 +174,7 @@ __global__ __launch_bounds__(THREADS, 8) void distill_row_kernel(DistillTop a) {
     patch_entries(a, c, out, lds, t);
 }
 
-// A row longer than a workgroup's registers (2048 x 128011 f32: 500 us; stretches of rows in workgroups of their
+// A row longer than a workgroup's registers (2048 x 128011 f32: 493 us; stretches of rows in workgroups of their
 // own, in a launch for the statistics, one for the losses and one for the gradient, 566 us): the workgroup sweeps
 // the row in stretches, every thread with a maximum and a sum of its own, joins them, and sweeps back
 // to write the gradient, from the last stretch, which it still holds, to the first.

@@ -7,6 +7,8 @@
 // found in the registers: numbers below a bound that at least `top` numbers reach are passed over, and
 // the few that are left are ranked.  Order: larger logit first, among equals the lower token, -0 = +0,
 // NaN behind -inf; so equal calls give equal bytes whatever order the candidates were found in.
+// Measured on 4096 x 32768 f32: 77 us = 7.0 TB/s without alternatives, 105 us with the top 64 (then bound by vector
+// issue: 672 instructions a wave instead of 353); gradient of 8192 x 128000 bf16 712 us = 5.9 TB/s.
 #include <hip/hip_runtime.h>
 
 #include <cmath>

@@ -414,6 +414,31 @@ def test_loss_gradients_by_differences(ops):
             assert abs((fn(up_z) - fn(down_z)) / (2 * step) - float(grad[row, c])) <= bound
 
 
+@pytest.mark.parametrize("temperature", [0.03, 60.0])
+@pytest.mark.parametrize("rows, vocab", [(5, 3001), (2, 70001)])
+def test_sharp_and_flat_temperatures(ops, rows, vocab, temperature):
+    g = generator(vocab)
+    z = logits_of(g, rows, vocab, torch.float32)
+    tokens = torch.randint(0, vocab, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    check_log_probs(ops, z, tokens, 10, temperature)
+
+
+def test_without_tokens_and_with_the_entropy_alone(ops):
+    g = generator(21)
+    z = logits_of(g, 6, 900, torch.float32)
+    r = ops.token_log_probs(z, top=5)
+    assert r.log_prob is None
+    whole = ops.token_log_probs(z, torch.zeros(6, dtype=torch.int32, device="cuda"), top=5)
+    for a, b in zip(r[1:], whole[1:]):
+        assert torch.equal(a, b)
+    up_h = torch.randn(6, generator=g, device="cuda")
+    got = ops.token_log_probs_backward(z, None, r.lse, r.entropy, None, up_h)
+    none = torch.full((6,), -1, dtype=torch.int32, device="cuda")
+    assert torch.equal(got, ops.token_log_probs_backward(z, none, r.lse, r.entropy, None, up_h))
+    want, p = rows64.token_log_probs_backward(z, none, None, up_h, 1.0)
+    rows64.close(got, want, up_h.double().abs()[:, None] * p * (math.log(900) + 12) * 600, 1, "grad")
+
+
 # ---- how they are called --------------------------------------------------------------------------
 def test_shapes_and_workspaces(ops):
     g = generator(3)
