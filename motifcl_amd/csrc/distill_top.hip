@@ -118,15 +118,14 @@ __device__ __forceinline__ void write_stretch(const GradientScale& c, T* out, in
         r.store(out, j, t, n, v);
     }
 }
-// All waves' gradient is in memory, past the point where a second store to an element could overtake the first.
-__device__ __forceinline__ void gradient_written() {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-}
-// The elements that the teacher's entries name, by the first wave, after gradient_written().
+// Once the whole row's gradient is written, the elements that the teacher's entries name, by the first wave.  All
+// threads call it: first every wave waits until its stores are in memory, for another wave stores some of the same
+// elements again, and a barrier alone waits for no store.
 template <typename T>
 __device__ __forceinline__ void patch_entries(const DistillTop& a, const GradientScale& c, T* out,
                                               const EntryScratch& lds, int t) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
     if (t >= 64 || c.zero) return;
     for (int at = t; at < a.top; at += 64) {
         const int id = lds.id[at];
@@ -170,7 +169,6 @@ __global__ __launch_bounds__(THREADS, 8) void distill_row_kernel(DistillTop a) {
     const GradientScale c(a, row, st.m, st.s, lds.sum);
     T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
     write_stretch<T, THREADS, ITERS>(c, out, n, r, t);
-    gradient_written();
     patch_entries(a, c, out, lds, t);
 }
 
@@ -233,7 +231,6 @@ __global__ __launch_bounds__(1024, 8) void distill_sweep_kernel(DistillTop a, in
         from = (i - 1) * length, n = length;
         r.load(logits + from, again(t), n);
     }
-    __syncthreads();
     patch_entries(a, c, out, lds, t);
 }
 template <typename T>
