@@ -286,6 +286,9 @@ __global__ __launch_bounds__(kLongThreads) void layer_norm_grad_x_long_kernel(
 // out[i] = sum over the partial rows, of the gain (blockIdx.y 0) and of the bias (1); a workgroup adds
 // 32 columns, 32 partial rows at a time with eight loads under way, and then the 32 sums in order.
 constexpr int kJoinColumns = 32, kJoinRows = 32;
+// Columns of one launch; wider rows go out as several, for at 1024 threads per 32 columns 2^27 columns would be the
+// 2^32 threads that no launch may have.
+constexpr int kMostJoinColumns = (int)kMostLaunchRows * kJoinColumns;
 __global__ __launch_bounds__(kJoinColumns* kJoinRows) void layer_norm_join_kernel(
     const float* partial_gain, const float* partial_bias, size_t partial_stride, int partials, float* grad_gain,
     float* grad_bias, int n) {
@@ -425,8 +428,13 @@ hipError_t backward(hipStream_t stream, const void* dv, size_t d_stride, const v
 #undef MCC_NORM_BACKWARD
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !join || (!pg && !pb)) return e;
-    hipLaunchKernelGGL(layer_norm_join_kernel, dim3((unsigned)((n + kJoinColumns - 1) / kJoinColumns), 2),
-                       dim3(kJoinColumns * kJoinRows), 0, stream, pg, pb, stride, (int)groups, grad_gain, grad_bias, n);
+    auto from = [](float* p, int column) { return p ? p + column : nullptr; };
+    for (int done = 0; done < n; done += kMostJoinColumns) {
+        const int part = n - done < kMostJoinColumns ? n - done : kMostJoinColumns;
+        hipLaunchKernelGGL(layer_norm_join_kernel, dim3((unsigned)((part + kJoinColumns - 1) / kJoinColumns), 2),
+                           dim3(kJoinColumns * kJoinRows), 0, stream, from(pg, done), from(pb, done), stride, (int)groups,
+                           from(grad_gain, done), from(grad_bias, done), part);
+    }
     return hipGetLastError();
 }
 
