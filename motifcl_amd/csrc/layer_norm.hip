@@ -2,7 +2,7 @@
 //   mean = sum x / n,  rstd = 1 / sqrt(sum (x - mean)^2 / n + eps),  y = (x - mean) rstd gain + bias
 //   h = dy gain,  xhat = (x - mean) rstd:  dx = rstd (h - sum h / n - xhat sum(h xhat) / n),
 //   dgain = sum over rows of dy xhat,  dbias = sum over rows of dy
-// All of it in binary32; x, y, dy and dx have one element type of 32 or 16 bits.  Bound by memory: a
+// All of it in binary32, long running sums in binary64; x, y, dy and dx have one element type of 32 or 16 bits.  Bound by memory: a
 // row is read once into registers, where the mean is known before the squares are summed (no
 // difference of large sums), and the backward pass adds its columns up in registers over all rows of a
 // workgroup, so that only one partial row a workgroup is written and added up by a second launch.  No
@@ -124,7 +124,9 @@ __global__ __launch_bounds__(THREADS* SLOTS) void layer_norm_kernel(const T* x, 
     }
 }
 
-// Rows longer than a workgroup's registers: three passes over the row, the later ones out of the caches.
+// Rows longer than a workgroup's registers: three passes over the row, the later ones out of the caches.  A thread
+// adds n / 1024 numbers, up to 2^20, one behind the other; in binary32 the error of such a sum grows with their number
+// (a row of 2^22 numbers 1.1: 700 half steps), so these sums are binary64 until the threads' are joined.
 constexpr int kLongThreads = 1024;
 template <typename T>
 __global__ __launch_bounds__(kLongThreads) void layer_norm_long_kernel(const T* x, size_t x_stride, const float* gain,
@@ -137,14 +139,17 @@ __global__ __launch_bounds__(kLongThreads) void layer_norm_long_kernel(const T* 
     const size_t row = blockIdx.x;
     const T* xr = x + row * x_stride;
     T* yr = y + row * y_stride;
-    float sum[1] = {0.0f}, squares[1] = {0.0f};
-    for (int i = t; i < n; i += kLongThreads) sum[0] += (float)xr[i];
+    double mine = 0.0;
+    for (int i = t; i < n; i += kLongThreads) mine += (double)(float)xr[i];
+    float sum[1] = {(float)mine};
     row_reduce<Sum, kWaves>(sum, slots, wave, lane);
     const float mean = sum[0] * inv_n;
+    mine = 0.0;
     for (int i = t; i < n; i += kLongThreads) {
         const float d = (float)xr[i] - mean;
-        squares[0] = fmaf(d, d, squares[0]);
+        mine += (double)d * (double)d;
     }
+    float squares[1] = {(float)mine};
     row_reduce<Sum, kWaves>(squares, slots + kWaves, wave, lane);
     const float rstd = inv_sqrt(squares[0] * inv_n + eps);
     if (t == 0) {
@@ -242,21 +247,22 @@ __global__ __launch_bounds__(THREADS* SLOTS) void layer_norm_backward_kernel(
 }
 
 // Rows longer than a workgroup's registers.  The columns' sums first (grad_x may overwrite grad_out):
-// a workgroup takes kLongThreads columns of every gridDim.y-th row; then the rows' gradient in two passes.
+// a workgroup takes kLongThreads columns of every gridDim.y-th row; then the rows' gradient in two passes.  Sums over
+// rows and over a thread's columns are binary64, as in the forward pass.
 template <typename T>
 __global__ __launch_bounds__(kLongThreads) void layer_norm_columns_long_kernel(
     const T* grad_out, size_t grad_out_stride, const T* x, size_t x_stride, const float* mean, const float* rstd,
     float* partial_gain, float* partial_bias, size_t partial_stride, size_t rows, int n) {
     const int i = blockIdx.x * kLongThreads + threadIdx.x;
     if (i >= n) return;
-    float dgain = 0.0f, dbias = 0.0f;
+    double dgain = 0.0, dbias = 0.0;
     for (size_t row = blockIdx.y; row < rows; row += gridDim.y) {
         const float d = (float)grad_out[row * grad_out_stride + i];
-        dgain = fmaf(d, ((float)x[row * x_stride + i] - mean[row]) * rstd[row], dgain);
-        dbias += d;
+        dgain += (double)d * (double)(((float)x[row * x_stride + i] - mean[row]) * rstd[row]);
+        dbias += (double)d;
     }
-    if (partial_gain) partial_gain[blockIdx.y * partial_stride + i] = dgain;
-    if (partial_bias) partial_bias[blockIdx.y * partial_stride + i] = dbias;
+    if (partial_gain) partial_gain[blockIdx.y * partial_stride + i] = (float)dgain;
+    if (partial_bias) partial_bias[blockIdx.y * partial_stride + i] = (float)dbias;
 }
 
 template <typename T>
@@ -269,12 +275,13 @@ __global__ __launch_bounds__(kLongThreads) void layer_norm_grad_x_long_kernel(
     const size_t row = blockIdx.x;
     const T *xr = x + row * x_stride, *dr = grad_out + row * grad_out_stride;
     const float mean = mean_in[row], rstd = rstd_in[row];
-    float sums[2] = {0.0f, 0.0f};
+    double sum_h = 0.0, sum_hx = 0.0;
     for (int i = t; i < n; i += kLongThreads) {
         const float h = (float)dr[i] * (gain ? gain[i] : 1.0f);
-        sums[0] += h;
-        sums[1] = fmaf(h, ((float)xr[i] - mean) * rstd, sums[1]);
+        sum_h += (double)h;
+        sum_hx += (double)h * (double)(((float)xr[i] - mean) * rstd);
     }
+    float sums[2] = {(float)sum_h, (float)sum_hx};
     row_reduce<Sum, kWaves>(sums, slots, t >> 6, t & 63);
     const float a = sums[0] * inv_n, b = sums[1] * inv_n;
     for (int i = t; i < n; i += kLongThreads) {  // grad_x may be grad_out or x: one thread owns an element

@@ -26,3 +26,55 @@ def test_column_gradients_of_the_widest_rows(ops):
         # x - mean, its product with rstd, the product with dy, the sum of the two rows
         rows64.close(dgain[at], (d * xhat).sum(0), (d.abs() * near).sum(0), 4, "dgain")
         rows64.close(dbias[at], d.sum(0), d.abs().sum(0), 1, "dbias")
+
+
+# Sums of a row that a workgroup's registers do not hold: a thread's own is rounded once, then a tree of 6 + 6 joins, the
+# rounded 1 / n and its product: at most 16 U of the mean magnitude, whatever the length.
+LONG_SUM = 16
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("spread", [0.0, 2.0 ** -5])
+def test_norm_of_long_rows_far_from_zero(ops, dtype, spread):
+    rows, cols, eps = 2, (1 << 22) + 3, 1e-5
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    x = (1.1 + spread * torch.randn(rows, cols, generator=g, device="cuda")).to(dtype)
+    y, mean, rstd = ops.layer_norm(x, None, None, eps)
+    want, want_mean, want_rstd = rows64.layer_norm(x, None, None, eps)
+    largest = x.double().abs().max(1).values
+    rows64.close(mean, want_mean, largest, LONG_SUM, "mean")
+    # a difference is off by the mean's error and its own rounding, the variance by twice that against the deviation,
+    # by its square (small here: below 2^-12 of itself, where the deviation is 0 it is compared with eps) and its sum
+    slack = (LONG_SUM + 1) * rows64.U * largest * want_rstd
+    relative = (LONG_SUM + 6) * rows64.U + 2 * slack
+    assert ((rstd.double() - want_rstd).abs() <= want_rstd * relative).all()
+    scale = (x.double() - want_mean[:, None]).abs() * want_rstd[:, None]
+    rows64.close(y, want, (scale * (relative[:, None] + 4 * rows64.U) + slack[:, None]) / rows64.U, 1, "y")
+
+
+def test_norm_gradient_of_long_rows_far_from_zero(ops):
+    rows, cols = 2, (1 << 22) + 3
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    x = torch.randn(rows, cols, generator=g, device="cuda")
+    dy = torch.full_like(x, 0.7)  # equal numbers round the same way every time
+    _, mean, rstd = ops.layer_norm(x)
+    dx, _, _ = ops.layer_norm_backward(dy, x, mean, rstd, bias=False)
+    want, _, _ = rows64.layer_norm_backward(dy, x, mean, rstd, None)
+    near = (x.double().abs() + mean.double().abs()[:, None]) * rstd.double()[:, None]
+    h = dy.double().abs()
+    # xhat within 3 U of |x| + |mean|; h - a - xhat b and its product with rstd: 5 roundings
+    scale = rstd.double()[:, None] * (h + h.mean(1, keepdim=True) + near * (h * near).mean(1, keepdim=True))
+    rows64.close(dx, want, scale, LONG_SUM + 10, "dx")
+
+
+def test_column_gradients_of_many_long_rows(ops):
+    # 1024 rows to each partial row of a matrix wider than the registers
+    rows, cols = 1 << 16, 16392
+    x = torch.ones(rows, cols, device="cuda")
+    dy = torch.full_like(x, 0.7)
+    mean, rstd = torch.full((rows,), 0.25, device="cuda"), torch.full((rows,), 0.75, device="cuda")
+    _, dgain, dbias = ops.layer_norm_backward(dy, x, mean, rstd, torch.ones(cols, device="cuda"), input_grad=False)
+    total = torch.full((cols,), float(dy[0, 0]) * rows, device="cuda", dtype=torch.float64)
+    # the thread's sum is rounded once, the partial rows are added in two steps and 31
+    rows64.close(dbias, total, total, 34, "dbias")
+    rows64.close(dgain, 0.5625 * total, total, 36, "dgain")
