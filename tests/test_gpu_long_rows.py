@@ -78,3 +78,20 @@ def test_column_gradients_of_many_long_rows(ops):
     # the thread's sum is rounded once, the partial rows are added in two steps and 31
     rows64.close(dbias, total, total, 34, "dbias")
     rows64.close(dgain, 0.5625 * total, total, 36, "dgain")
+
+
+def test_distillation_of_rows_of_equal_logits(ops):
+    # 534 stretches of 65536: one running sum of equal numbers in binary32 would be off by thousands of roundings
+    vocab, rows = 35000003, 2
+    z = torch.full((rows, vocab), -0.357, device="cuda", dtype=torch.bfloat16)
+    z[:, :65536] = 0.0  # every thread's largest
+    ids = torch.tensor([[5, vocab - 1]] * rows, dtype=torch.int32, device="cuda")
+    loss, grad = ops.distill_top(z, ids, torch.zeros(rows, 2, device="cuda"))
+    want_loss, want, _, _ = rows64.distill_top(z, ids, torch.zeros(rows, 2, device="cuda"), None, 1.0)
+    # e^d with |d| < 1 is off by 7 U, a thread's 64 of them by 64 U, 12 joins, the rescaling: s within 90 U of itself;
+    # log p by that, the rounding of log s (18 U at most) and of their difference
+    rows64.close(loss, want_loss, 1.0, 150, "loss")
+    # p = e^d / s, rounded with T, q and the product; at the two entries q is subtracted
+    entries = torch.zeros(vocab, dtype=torch.float64, device="cuda")
+    entries[ids[0].long()] = 1.0
+    rows64.close(grad, want, want.abs() + entries, 105, "grad")
