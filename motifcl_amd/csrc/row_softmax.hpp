@@ -24,14 +24,23 @@ struct SoftmaxStats {
 // What a maximum is subtracted as: 0 where there is none, so that -inf - (-inf) does not arise.
 __device__ __forceinline__ float shift_of(float m) { return m == -__builtin_inff() ? 0.0f : m; }
 
-// a joined to b; the order of the operands is the order of the stretches
-__device__ __forceinline__ SoftmaxStats join_stats(SoftmaxStats a, SoftmaxStats b, float k) {
-    const float m = fmaxf(a.m, b.m), base = shift_of(m);
-    const float da = (a.m - base) * k, db = (b.m - base) * k;
-    const float ra = exp2_of(da), rb = exp2_of(db);
-    // an empty stretch has d = -inf: its sums are zero and stay so
-    return {m, ra * a.s + rb * b.s, ra * (a.u + a.s * fmaxf(da, -1e4f)) + rb * (b.u + b.s * fmaxf(db, -1e4f))};
-}
+// A row's stretches, joined in their order.  The sums are binary64: a row may have 32768 stretches, and the error of a
+// sum in binary32 grows with their number (16385 equal ones: 2300 half steps).
+struct JoinedStats {
+    float m;
+    double s, u;
+    __device__ __forceinline__ explicit JoinedStats(const SoftmaxStats& a) : m(a.m), s(a.s), u(a.u) {}
+    __device__ __forceinline__ void join(const SoftmaxStats& b, float k) {
+        const float most = fmaxf(m, b.m), base = shift_of(most);
+        const float da = (m - base) * k, db = (b.m - base) * k;
+        const double ra = exp2_of(da), rb = exp2_of(db);
+        // an empty stretch has d = -inf: its sums are zero and stay so
+        u = ra * (u + s * (double)fmaxf(da, -1e4f)) + rb * ((double)b.u + (double)b.s * (double)fmaxf(db, -1e4f));
+        s = ra * s + rb * (double)b.s;
+        m = most;
+    }
+    __device__ __forceinline__ SoftmaxStats stats() const { return {m, (float)s, (float)u}; }
+};
 
 // scale is k above; slots: 3 * WAVES floats of LDS that no wave still reads
 template <typename ROW, int WAVES, int ITERS>

@@ -359,9 +359,9 @@ __global__ __launch_bounds__(kJoinThreads) void token_log_probs_join_kernel(Toke
     const size_t row = blockIdx.x;
     float token_logit = 0.0f;
     const bool has_token = t == 0 && token_of<T>(a, row, token_logit);
-    SoftmaxStats st = stats[row * segments];
-    for (int i = 1; i < segments; ++i) st = join_stats(st, stats[row * segments + i], a.log2_scale);
-    const RowResult result = finish_row(a, row, st, token_logit, has_token, t == 0);
+    JoinedStats joined(stats[row * segments]);
+    for (int i = 1; i < segments; ++i) joined.join(stats[row * segments + i], a.log2_scale);
+    const RowResult result = finish_row(a, row, joined.stats(), token_logit, has_token, t == 0);
     if (a.top == 0 || (!a.top_ids && !a.top_log_probs)) return;
     const uint64_t* entries = best + row * segments * a.top;
     const int all = segments * a.top, nth = (a.top + segments - 1) / segments;

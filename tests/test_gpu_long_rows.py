@@ -1,6 +1,8 @@
 """The row-wise operators on rows, vocabularies and batches far longer than a workgroup's registers.
 
 A rounding of binary32 is U = 2^-24 of the value; `steps` below counts the roundings on the longest path of a sum."""
+import math
+
 import pytest
 
 from . import rows64
@@ -95,3 +97,18 @@ def test_distillation_of_rows_of_equal_logits(ops):
     entries = torch.zeros(vocab, dtype=torch.float64, device="cuda")
     entries[ids[0].long()] = 1.0
     rows64.close(grad, want, want.abs() + entries, 105, "grad")
+
+
+def test_log_probs_of_the_most_stretches(ops):
+    # 16385 stretches of nearly equal sums
+    vocab = (1 << 29) + 3
+    z = torch.full((1, vocab), -0.5, device="cuda")
+    z[:, ::16384] = 0.0  # every stretch's largest
+    tokens = torch.tensor([vocab - 1], dtype=torch.int32, device="cuda")
+    r = ops.token_log_probs(z, tokens)
+    ones = (vocab + 16383) // 16384
+    e = math.exp(-0.5)
+    s, u = ones + (vocab - ones) * e, -0.5 * (vocab - ones) * e
+    # a stretch's s and u: e^d within 6 U, a thread's 32 of them 32 U, 12 joins; then log s (20 at most) and its sum
+    for got, want in ((r.lse, math.log(s)), (r.log_prob, -0.5 - math.log(s)), (r.entropy, math.log(s) - u / s)):
+        assert abs(float(got[0]) - want) <= (2 * 50 + 2 * 21) * rows64.U
