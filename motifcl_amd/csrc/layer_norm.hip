@@ -10,6 +10,7 @@
 // that shape 140 us = 5.7 TB/s; 8192 x 288 f32 forward 5.8 us, backward 10.0 + 3.8 us, both shorter than the calls.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "launch.hpp"
@@ -291,7 +292,7 @@ __global__ __launch_bounds__(kLongThreads) void layer_norm_grad_x_long_kernel(
 }
 
 // out[i] = sum over the partial rows, of the gain (blockIdx.y 0) and of the bias (1); a workgroup adds
-// 32 columns, 32 partial rows at a time with eight loads under way, and then the 32 sums in order.
+// 32 columns, 32 partial rows at a time with eight loads under way, and then the 32 sums in order, all in binary64.
 constexpr int kJoinColumns = 32, kJoinRows = 32;
 // Columns of one launch; wider rows go out as several, for at 1024 threads per 32 columns 2^27 columns would be the
 // 2^32 threads that no launch may have.
@@ -299,12 +300,12 @@ constexpr int kMostJoinColumns = (int)kMostLaunchRows * kJoinColumns;
 __global__ __launch_bounds__(kJoinColumns* kJoinRows) void layer_norm_join_kernel(
     const float* partial_gain, const float* partial_bias, size_t partial_stride, int partials, float* grad_gain,
     float* grad_bias, int n) {
-    __shared__ float sums[kJoinRows][kJoinColumns];
+    __shared__ double sums[kJoinRows][kJoinColumns];
     const float* p = blockIdx.y ? partial_bias : partial_gain;
     float* out = blockIdx.y ? grad_bias : grad_gain;
     if (!out) return;
     const int c = threadIdx.x % kJoinColumns, r = threadIdx.x / kJoinColumns, i = blockIdx.x * kJoinColumns + c;
-    float a = 0.0f;
+    double a = 0.0;
     if (i < n) {
         int row = r;
         for (; row + 7 * kJoinRows < partials; row += 8 * kJoinRows) {
@@ -312,15 +313,15 @@ __global__ __launch_bounds__(kJoinColumns* kJoinRows) void layer_norm_join_kerne
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = p[(row + k * kJoinRows) * partial_stride + i];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) a += v[k];
+            for (int k = 0; k < 8; ++k) a += (double)v[k];
         }
-        for (; row < partials; row += kJoinRows) a += p[row * partial_stride + i];
+        for (; row < partials; row += kJoinRows) a += (double)p[row * partial_stride + i];
     }
     sums[r][c] = a;
     __syncthreads();
     if (r == 0 && i < n) {
         for (int k = 1; k < kJoinRows; ++k) a += sums[k][c];
-        out[i] = a;
+        out[i] = (float)a;
     }
 }
 
@@ -340,11 +341,15 @@ BackwardShape backward_shape(int n, int vec) {
 }
 constexpr size_t kLongColumnRows = 64;  // partial rows where rows do not fit the registers
 
-// Workgroups of the backward kernel, each of which writes a partial row: two of 512 threads a CU.
+// Workgroups of the backward kernel, each of which writes a partial row: two of 512 threads a CU, and more where a thread
+// would add more than 256 rows to its column's sum, whose error in binary32 grows with their number (8192 equal ones:
+// 700 half steps).
+constexpr size_t kMostRowsOfASum = 256;
 size_t backward_groups(size_t rows, int n, int vec) {
     const BackwardShape s = backward_shape(n, vec);
     if (s.threads == 0) return rows < kLongColumnRows ? rows : kLongColumnRows;
-    const size_t groups = (rows + s.slots - 1) / s.slots, most = s.threads == 1024 ? 256 : 512;
+    const size_t groups = (rows + s.slots - 1) / s.slots, resident = s.threads == 1024 ? 256 : 512;
+    const size_t most = std::max(resident, (groups + kMostRowsOfASum - 1) / kMostRowsOfASum);
     return groups < most ? groups : most;
 }
 

@@ -112,3 +112,16 @@ def test_log_probs_of_the_most_stretches(ops):
     # a stretch's s and u: e^d within 6 U, a thread's 32 of them 32 U, 12 joins; then log s (20 at most) and its sum
     for got, want in ((r.lse, math.log(s)), (r.log_prob, -0.5 - math.log(s)), (r.entropy, math.log(s) - u / s)):
         assert abs(float(got[0]) - want) <= (2 * 50 + 2 * 21) * rows64.U
+
+
+def test_column_gradients_of_very_many_rows(ops):
+    # 33 million rows: no thread adds more than 256 of them up in binary32
+    rows, cols = (1 << 25) + 3, 16
+    x = torch.ones(rows, cols, device="cuda")
+    dy = torch.full_like(x, 0.7)
+    mean, rstd = torch.full((rows,), 0.25, device="cuda"), torch.full((rows,), 0.75, device="cuda")
+    _, dgain, dbias = ops.layer_norm_backward(dy, x, mean, rstd, torch.ones(cols, device="cuda"), input_grad=False)
+    total = torch.full((cols,), float(dy[0, 0]) * rows, device="cuda", dtype=torch.float64)
+    # a thread's 256 rows, three joins of a workgroup's eight, the products; the partial rows' sum is rounded once
+    rows64.close(dbias, total, total, 259, "dbias")
+    rows64.close(dgain, 0.5625 * total, total, 261, "dgain")
