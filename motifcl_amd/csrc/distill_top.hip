@@ -23,7 +23,7 @@ constexpr int kHeld = kMostTop / 64;
 struct Entries {
     int id[kHeld];                // -1: none
     float z[kHeld], y[kHeld];     // the student's logit at id, the teacher's
-    float q[kHeld], log_q[kHeld];
+    float q[kHeld], t_log_q[kHeld];  // q and T log q
     float sum;                    // of q: 1, 0 without entries, NaN where the teacher has no distribution
 };
 template <typename T>
@@ -49,15 +49,15 @@ __device__ __forceinline__ void weigh_entries(const DistillTop& a, Entries& e) {
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
-        e.log_q[i] = (e.y[i] - largest) * a.inv_temperature;
-        e.q[i] = exp2_of(e.log_q[i] * kLog2E);
+        e.t_log_q[i] = e.y[i] - largest;
+        e.q[i] = exp2_of(e.t_log_q[i] * a.inv_temperature * kLog2E);
         sum += e.q[i];
     }
     sum = wave_reduce<Sum>(sum);
     const float log_sum = logf(sum), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
-        e.log_q[i] -= log_sum;
+        e.t_log_q[i] -= a.temperature * log_sum;
         e.q[i] *= inv;
     }
     e.sum = sum == 0.0f ? 0.0f : sum * inv;
@@ -66,30 +66,31 @@ __device__ __forceinline__ void weigh_entries(const DistillTop& a, Entries& e) {
 // be replaced by the gradient.
 struct EntryScratch {
     int id[kMostTop];
-    float q[kMostTop], log_q[kMostTop], z[kMostTop];
+    float q[kMostTop], t_log_q[kMostTop], z[kMostTop];
     float sum;
     __device__ __forceinline__ void put(const Entries& e, int lane) {
 #pragma unroll
         for (int i = 0; i < kHeld; ++i) {
             id[lane + 64 * i] = e.id[i];
             q[lane + 64 * i] = e.q[i];
-            log_q[lane + 64 * i] = e.log_q[i];
+            t_log_q[lane + 64 * i] = e.t_log_q[i];
             z[lane + 64 * i] = e.z[i];
         }
         if (lane == 0) sum = e.sum;
     }
 };
 
-// T^2 sum q (log q - log p), in every lane of the first wave
+// T sum q (T log q - T log p), in every lane of the first wave: neither T^2 nor a difference of logits over T is formed,
+// of which a small T would leave 0 and infinity.
 __device__ __forceinline__ float loss_of(const DistillTop& a, const EntryScratch& e, float m, float s, int lane) {
-    const float log_s = logf(s);
+    const float t_log_s = a.temperature * logf(s);
     float sum = 0.0f;
 #pragma unroll
     for (int i = lane; i < kMostTop; i += 64) {
-        const float log_p = s == 0.0f ? -__builtin_inff() : (e.z[i] - m) * a.inv_temperature - log_s;
-        if (e.id[i] >= 0 && e.q[i] != 0.0f) sum += e.q[i] * (e.log_q[i] - log_p);
+        const float t_log_p = s == 0.0f ? -__builtin_inff() : e.z[i] - m - t_log_s;
+        if (e.id[i] >= 0 && e.q[i] != 0.0f) sum += e.q[i] * (e.t_log_q[i] - t_log_p);
     }
-    return a.temperature * a.temperature * wave_reduce<Sum>(sum);
+    return a.temperature * wave_reduce<Sum>(sum);
 }
 
 // The gradient without the teacher's entries is c 2^((z - base) k).
