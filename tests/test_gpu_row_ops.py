@@ -1,9 +1,11 @@
 """Layer norm, token log probabilities and the distillation loss against their definitions in 64 bits.
 
-Bounds, in half steps of binary32 (U = 2^-24).  A thread adds at most 32 numbers and a tree of at most 6 + 16
-joins its sum, so a sum is off by at most 64 U of the sum of magnitudes.  e^d is off by (3 |d| + 4) U of itself: the
-difference, the temperature's reciprocal and its product, the hardware's exponential; with |d| e^d <= 1 a sum of
-e^d, which is at least 1, is off by at most (64 + 3 ln(vocab) + 4) U <= 128 U of itself, and its logarithm by that."""
+Bounds, in half steps of binary32 (U = 2^-24).  A thread adds at most 64 numbers (32 of f32) one behind the other and at
+most 12 joins follow, so a sum is off by at most 76 U (f32: 44 U) of the sum of magnitudes; the norm's tests hold all of
+them to 64 U.  Longer running sums, of long rows and of swept rows, are binary64 between stretches of as many numbers.
+e^d is off by (3 |d| + 4) U of itself: the difference, the temperature's reciprocal and its product, the hardware's
+exponential; with |d| e^d <= 1 a sum of e^d, which is at least 1, is off by at most (76 + 3 ln(vocab) + 4) U of itself,
+128 U up to vocabularies of 8 million, and its logarithm by that."""
 import math
 
 import pytest
