@@ -368,9 +368,10 @@ int mcc_adam_update_f32(void* stream, float* param, size_t param_nbytes, const f
  *
  * Large tensors are rows of elements of one type, MCC_ELEMENT_*, aligned to the element; a stride counts
  * the elements from the start of a row to that of the next (at least the row's length).  Whatever the
- * type, everything is computed in binary32 and a result is rounded to the type once.  An output may
- * replace an input of the same type where that is said (same pointer, same stride); any other overlap of
- * the large tensors is refused.  Equal calls give equal bytes.  Rows hold at most 2^30 elements.
+ * type, everything is computed in binary32 (sums whose error would grow with the length of a row or the
+ * number of rows in binary64) and a result is rounded to the type once.  An output may replace an input of
+ * the same type where that is said (same pointer, same stride); any other overlap of the large tensors is
+ * refused.  Equal calls give equal bytes.  Rows hold at most 2^30 elements.
  * Nothing is allocated and nothing is kept between calls: all entry points may be captured into a graph.
  * Workspaces are aligned to 16 bytes and belong to the call until it has run; their sizes depend on the
  * arguments of the query alone and may be 0 (then the pointer may be null).
@@ -429,10 +430,11 @@ int mcc_token_log_probs(void* stream, const void* logits, size_t logits_nbytes, 
  *   ((token == j) - p_j) * grad_log_prob - p_j (log p_j + entropy) * grad_entropy,  over temperature.
  * With grad_log_prob = -1 / n it is the gradient of the mean cross entropy.  Ignored positions take no
  * grad_log_prob.  Rows whose upstream gradients are zero and rows of -inf alone get zeros whatever their
- * logits hold.  p is taken as exp(logit / temperature - lse), so lse has to hold it: in a row whose
+ * logits hold.  p is taken as exp(logit / temperature - lse), so lse has to hold it: p's relative error grows
+ * with |lse|, by 2^-24 |lse| (logits over the temperature in the thousands: 2^-12), and in a row whose
  * largest logit is so far from zero that its lse rounds log sum away (beyond 2^24, as the type's lowest
- * value used as a mask for the whole row) the gradient is not that of the uniform row.  grad_logits may
- * replace logits.
+ * value used as a mask for the whole row) the gradient is not that of the uniform row; where lse leaves the
+ * range of binary32 it is 0 (-inf) or NaN (+inf).  grad_logits may replace logits.
  */
 int mcc_token_log_probs_backward(void* stream, const void* logits, size_t logits_nbytes, size_t logits_stride,
                                  const int32_t* tokens, size_t tokens_nbytes, const float* lse, size_t lse_nbytes,

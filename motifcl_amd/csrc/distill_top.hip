@@ -4,8 +4,8 @@
 // sum q is 1, or 0 in a row without entries.  One workgroup a row, one launch.  Bound by memory: the logits are
 // read once and the gradient is written once where the workgroup's registers hold the row; a longer row is read a
 // second time, as far as the registers and caches do not hold it.  The teacher's entries change `top` elements of a
-// row: the gradient is written without them first and those elements are written again behind a barrier, each by
-// the first of the entries that name it.  Measured: 4096 x 32768 f32 190 us = 5.7 TB/s; 2048 x 128011 f32 493 us, of
+// row: the gradient is written without them first, and once all of it is in memory those elements are written again, each
+// by the first of the entries that name it.  Measured: 4096 x 32768 f32 190 us = 5.7 TB/s; 2048 x 128011 f32 493 us, of
 // whose 2.9 GB 0.8 are the second read.
 #include <hip/hip_runtime.h>
 

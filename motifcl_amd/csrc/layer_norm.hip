@@ -127,7 +127,8 @@ __global__ __launch_bounds__(THREADS* SLOTS) void layer_norm_kernel(const T* x, 
 
 // Rows longer than a workgroup's registers: three passes over the row, the later ones out of the caches.  A thread
 // adds n / 1024 numbers, up to 2^20, one behind the other; in binary32 the error of such a sum grows with their number
-// (a row of 2^22 numbers 1.1: 700 half steps), so these sums are binary64 until the threads' are joined.
+// (a row of 2^22 numbers 1.1: 700 half steps), so these sums are binary64 until the threads' are joined.  One element an
+// access and a workgroup a row: 2048 x 50000 f32 forward 322 us = 2.5 TB/s, backward 566 us; two rows of 2^22 3.7 ms.
 constexpr int kLongThreads = 1024;
 template <typename T>
 __global__ __launch_bounds__(kLongThreads) void layer_norm_long_kernel(const T* x, size_t x_stride, const float* gain,

@@ -42,7 +42,8 @@ struct JoinedStats {
     __device__ __forceinline__ SoftmaxStats stats() const { return {m, (float)s, (float)u}; }
 };
 
-// scale is k above; slots: 3 * WAVES floats of LDS that no wave still reads
+// scale is k above; slots: 3 * WAVES floats of LDS that no wave still reads.  A thread adds its kVec * ITERS numbers, 32
+// of f32 and at most 64 of 16 bits, one behind the other, and at most 12 joins follow.
 template <typename ROW, int WAVES, int ITERS>
 __device__ __forceinline__ SoftmaxStats stats_of(ROW& r, float scale, float* slots, int wave, int lane,
                                                  float& thread_max) {

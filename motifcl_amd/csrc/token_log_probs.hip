@@ -56,10 +56,14 @@ __device__ __forceinline__ int total_of(int wave_count, float (&totals)[2][WAVES
 }
 
 // A number that at least `top` of the workgroup's numbers reach.  The threads' maxima are joined over groups
-// of neighbouring lanes, 256 groups a workgroup (64 for a workgroup of one wave), and the first wave finds the
-// top-th largest of the groups' maxima, each of which is a number of its own, by bisection over the leading 20
-// bits of its key: a compare and a population count a bit.  Of random numbers about 256 ln(256 / (256 - top))
-// reach it: 75 for the top 64.
+// of neighbouring lanes, and the first wave finds the top-th largest of the groups' maxima, each of which is a
+// number of its own, by bisection over the leading 20 bits of its key: a compare and a population count a bit.
+// Of random numbers about G ln(G / (G - top)) reach it, G groups: 256 from four waves on (75 for the top 64, 177 for
+// the top 128), 128 of two waves, 64 of one (24 for the top 20, 89 for the top 48, 220 for the top 62).  Where top
+// comes near G more numbers reach it than are listed, and beyond G it is -inf: those rows go to select_among_ties,
+// ties or not.  That is one-wave rows (up to 2048 f32, 4096 16-bit numbers) from about the top 60 on and two-wave rows
+// (16-bit, up to 8192) from about the top 126: 16384 x 3001 bf16 takes 45 us for the top 20, 79 for 48, 182 for 62 and
+// 242 for 128, 16384 x 2000 f32 29, 64, 166 and 148, 16384 x 8000 bf16 74, 90, 107 and 762.
 template <int WAVES>
 __device__ __forceinline__ float lower_bound_of(float thread_max, int top, TopScratch<WAVES>& lds, int t, int wave, int lane) {
     constexpr int kLanes = WAVES > 4 ? WAVES / 4 : 1, kGroups = WAVES * 64 / kLanes, kHeld = kGroups / 64;
@@ -92,8 +96,8 @@ __device__ __forceinline__ float lower_bound_of(float thread_max, int top, TopSc
     return bound <= kKeyLowest ? -__builtin_inff() : of_key(bound);
 }
 
-// The `top` candidates of a stretch into lds.list[0 .. top) when too many numbers (ties, as of masked
-// logits) reach the bound, or too few (NaN): the top-th largest number, the numbers above it, and the
+// The `top` candidates of a stretch into lds.list[0 .. top) when too many numbers reach the bound (ties, as of masked
+// logits, or few groups) or too few (NaN): the top-th largest number, the numbers above it, and the
 // first of those equal to it.  The smallest number that reaches the bound is tried first: in rows with
 // fewer allowed tokens than `top` it is what the others were masked with (4096 x 32768 f32, 16 tokens allowed,
 // top 64: 143 us against 107 us without masks; 330 us before it was tried first and NaN were looked for only
@@ -302,7 +306,8 @@ __global__ __launch_bounds__(THREADS, 8) void token_log_probs_kernel(TokenLogPro
     __shared__ float slots[3 * kWaves];
     __shared__ TopScratch<TOP ? kWaves : 1> lds;
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
-    if constexpr (TOP) {  // a barrier of the statistics lies between this and its use
+    // between this and its use lies a barrier of the statistics, or there is one wave, whose LDS accesses keep their order
+    if constexpr (TOP) {
         if (t == 0) lds.count = 0;
         for (int i = t; i < lds.kCandidates; i += THREADS) lds.rank[i] = 0;
     }
