@@ -383,7 +383,8 @@ int mcc_adam_update_f32(void* stream, float* param, size_t param_nbytes, const f
 /*
  * y = (x - mean) * rstd * gain + bias with the row's mean and rstd = 1 / sqrt(variance + eps), the
  * variance being the mean of the squared differences.  gain and bias (cols floats) may be null: 1 and 0.
- * mean and rstd (rows floats), which the backward pass needs, may be null.  y may replace x.
+ * mean and rstd (rows floats), which the backward pass needs, may be null.  y may replace x.  Squared
+ * differences have to lie in the range of binary32: beyond 2^64 from the mean rstd is 0 and y the bias.
  */
 int mcc_layer_norm(void* stream, const void* x, size_t x_nbytes, size_t x_stride, const float* gain, size_t gain_nbytes,
                    const float* bias, size_t bias_nbytes, void* y, size_t y_nbytes, size_t y_stride, float* mean,
